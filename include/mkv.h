@@ -476,6 +476,124 @@ MKV_API int mkv_decode_metadata(const int32_t* packed, int32_t num_seqs, int32_t
                                 int32_t block_size, int64_t* slot_mapping, int64_t* context_lens,
                                 void* stream);
 
+/* ------------------------------------------------------------------------------------
+ * Decode steps over trees of drafted tokens (speculative decoding). No reference
+ * counterpart: the reference decodes one token per sequence and step. Sequence b of the
+ * step has prefix_lens[b] cached tokens and the drafted nodes that are rows
+ * [cu_seqlens_q[b], cu_seqlens_q[b+1]) of the step's arrays; node 0 is the tree's root (the
+ * last token that is certain) and parents[row] the index of a node's parent within its own
+ * tree, lower than the node's, or -1. A step runs mkv_tree_metadata, the model (append,
+ * mkv_paged_tree_attention per layer), mkv_tree_accept, mkv_move_kv_rows.
+ * ---------------------------------------------------------------------------------- */
+
+/*
+ * Metadata of the step, on the device (the counterpart of mkv_decode_metadata). Node i of
+ * sequence b is cached at position prefix_lens[b] + i:
+ *   slot_mapping[row] = its cache slot, -1 where the block table has no page
+ *   positions[row]    = prefix_lens[b] + its depth (the position for rotary embedding)
+ *   context_lens[b]   = prefix_lens[b] + nodes
+ *   tree_mask[row]    = mask_words 64-bit words: bit j % 64 of word j / 64 is set for the
+ *                       node itself and its ancestors j
+ * Rows of no sequence (padding before cu_seqlens_q[0] or behind the last) get slot -1,
+ * position 0 and an empty mask. A parent that is neither -1 nor lower than its node counts
+ * as -1; a node past 64 * mask_words gets slot -1 and an empty mask; both are counted in
+ * *invalid_count when it is non-NULL. mask_words is 1 to 16.
+ */
+MKV_API int mkv_tree_metadata(const void* parents, int32_t parents_index_type, const void* cu_seqlens_q,
+                              int32_t cu_seqlens_index_type, const void* prefix_lens,
+                              int32_t prefix_lens_index_type, const void* block_tables,
+                              int32_t block_table_index_type, int64_t block_table_stride_seq,
+                              int32_t max_num_blocks, int32_t block_size, int32_t num_seqs,
+                              int64_t total_q, int32_t mask_words, int64_t* slot_mapping,
+                              int64_t* context_lens, int64_t* positions, uint64_t* tree_mask,
+                              int32_t* invalid_count, void* stream);
+
+/*
+ * Attention of every tree's nodes over the paged cache. query (total_q, num_heads,
+ * head_dim); context_lens[b] includes the sequence's nodes, whose K/V must have been
+ * appended as its last n_b = cu_seqlens_q[b+1] - cu_seqlens_q[b] cached tokens. Row i of
+ * sequence b sees every token t < context_lens[b] - n_b, and the token of node j when bit j
+ * of its row of tree_mask (mask_words 64-bit words, rows mask_stride_token words apart) is
+ * set, whatever the mask's shape: the row's own node and its ancestors for a tree.
+ *     out[row, h] = softmax_t(scale * query[row, h] . K[t, kvh(h)]) V[t, kvh(h)]
+ * over what it sees, in fp32, kvh(h) = h / (num_heads / num_kv_heads). A row that sees
+ * nothing gives zeros. Tokens on a page entry that is -1 or out of range, or past
+ * max_num_blocks * block_size, are skipped. Rows of no sequence are left as they are.
+ * K/V that a row does not see may hold anything (infinities and NaN included).
+ * Caches: the query's dtype (bf16, f16, f32), FP8_E4M3 with k_scale / v_scale (one float
+ * each) or with k_scales / v_scales per (page, row, kv head), INT8 with k_scales /
+ * v_scales. head_dim is a multiple of 16, at most 256. query rows may have any strides
+ * (head_dim contiguous). workspace: 16-byte aligned, at least
+ * mkv_paged_tree_workspace_bytes(...), its contents on entry do not matter; calls that may
+ * overlap on the GPU need workspaces of their own.
+ */
+MKV_API size_t mkv_paged_tree_workspace_bytes(int32_t num_seqs, int64_t total_q, int32_t num_heads,
+                                              int32_t num_kv_heads, int32_t head_dim, int32_t q_dtype,
+                                              int32_t cache_dtype);
+MKV_API int mkv_paged_tree_attention(
+    const void* query, int64_t q_stride_token, int64_t q_stride_head, int32_t q_dtype,
+    const void* k_cache, const void* v_cache, int32_t cache_dtype, const float* k_scale,
+    const float* v_scale, const float* k_scales, const float* v_scales, int64_t num_blocks,
+    int32_t block_size, const void* block_tables, int32_t block_table_index_type,
+    int64_t block_table_stride_seq, int32_t max_num_blocks, const void* context_lens,
+    int32_t context_lens_index_type, const void* cu_seqlens_q, int32_t cu_seqlens_index_type,
+    const uint64_t* tree_mask, int64_t mask_stride_token, int32_t mask_words, int32_t num_seqs,
+    int64_t total_q, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim, float scale,
+    void* out, int64_t out_stride_token, int64_t out_stride_head, void* workspace,
+    size_t workspace_bytes, void* stream);
+
+/*
+ * Verification of the drafted tokens. draft_tokens[row] is the token of a node,
+ * target_tokens[row] the token that the target model puts after it. The accepted path
+ * starts at node 0; after node c comes its lowest-numbered child d with draft_tokens[d] ==
+ * target_tokens[c], until there is none or max_path nodes are taken. Per sequence:
+ *   num_accepted[b]         nodes of the path (0 for a sequence without nodes)
+ *   accepted_nodes[b, k]    (max_path, -1 padded) the path
+ *   tokens[b, k]            (max_path, -1 padded) target_tokens along it: the step's new
+ *                           tokens, the last of them not drafted
+ *   context_lens[b]         prefix_lens[b] + num_accepted[b]: cached tokens to keep
+ *   src_slots / dst_slots   (max_path) for mkv_move_kv_rows: node k of the path moves from
+ *                           its slot to that of position prefix_lens[b] + k; -1 where it
+ *                           is there already or k is past the path
+ */
+MKV_API int mkv_tree_accept(const void* draft_tokens, const void* target_tokens, int32_t token_index_type,
+                            const void* parents, int32_t parents_index_type, const void* cu_seqlens_q,
+                            int32_t cu_seqlens_index_type, const void* prefix_lens,
+                            int32_t prefix_lens_index_type, const void* block_tables,
+                            int32_t block_table_index_type, int64_t block_table_stride_seq,
+                            int32_t max_num_blocks, int32_t block_size, int32_t num_seqs, int64_t total_q,
+                            int32_t max_path, int32_t* num_accepted, int32_t* accepted_nodes,
+                            int64_t* tokens, int64_t* context_lens, int64_t* src_slots,
+                            int64_t* dst_slots, void* stream);
+
+/*
+ * Copies inside the cache, over all layers, K and V and (when given) the per-(page, row, kv
+ * head) scales, in one launch. k_cache / v_cache point at layer 0, (num_blocks, block_size,
+ * num_kv_heads, head_dim) each, layer_stride elements from layer to layer; k_scales /
+ * v_scales likewise (num_blocks, block_size, num_kv_heads), scale_layer_stride apart, or
+ * both NULL. A token's row (num_kv_heads x head_dim values) must be a multiple of 16 bytes.
+ *
+ * mkv_copy_kv_pages: page src_pages[i] to page dst_pages[i], i = 0 .. num_pairs - 1 (a fork's
+ * own copy of a shared page, compaction). The copies are made in order: one that reads a
+ * page that an earlier one wrote sees what was written.
+ * mkv_move_kv_rows: row src_slots[g, i] to dst_slots[g, i] for num_groups x moves_per_group
+ * moves (contiguous), in order within a group. Groups run side by side: what one writes no
+ * other may read or write (sequences write to pages of their own).
+ * A pair with a negative entry is no copy; one with an entry past the cache is skipped and
+ * counted in *invalid_count when that is non-NULL.
+ */
+MKV_API int mkv_copy_kv_pages(void* k_cache, void* v_cache, int32_t cache_dtype, int32_t num_layers,
+                              int64_t layer_stride, int64_t num_blocks, int32_t block_size,
+                              int32_t num_kv_heads, int32_t head_dim, float* k_scales, float* v_scales,
+                              int64_t scale_layer_stride, const void* src_pages, const void* dst_pages,
+                              int32_t index_type, int64_t num_pairs, int32_t* invalid_count, void* stream);
+MKV_API int mkv_move_kv_rows(void* k_cache, void* v_cache, int32_t cache_dtype, int32_t num_layers,
+                             int64_t layer_stride, int64_t num_blocks, int32_t block_size,
+                             int32_t num_kv_heads, int32_t head_dim, float* k_scales, float* v_scales,
+                             int64_t scale_layer_stride, const void* src_slots, const void* dst_slots,
+                             int32_t index_type, int32_t num_groups, int32_t moves_per_group,
+                             int32_t* invalid_count, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

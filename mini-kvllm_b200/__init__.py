@@ -14,13 +14,16 @@ from .layers.attention import (
     flash_attention_prefill,
     paged_attention_decode,
     paged_attention_decode_quantized,
+    paged_attention_tree,
     store_kvcache,
     store_kvcache_fp8,
 )
+from .engine.kv_cache import copy_kv_pages, move_kv_rows, tree_accept, tree_metadata
 from .utils.context import Context, get_context, reset_context, set_context
 
 __all__ = [
-    "Attention", "Context", "LIB_PATH", "MkvError", "flash_attention_prefill", "get_context", "load",
-    "paged_attention_decode", "paged_attention_decode_quantized", "reset_context",
-    "set_context", "store_kvcache", "store_kvcache_fp8",
+    "Attention", "Context", "LIB_PATH", "MkvError", "copy_kv_pages", "flash_attention_prefill",
+    "get_context", "load", "move_kv_rows", "paged_attention_decode",
+    "paged_attention_decode_quantized", "paged_attention_tree", "reset_context", "set_context",
+    "store_kvcache", "store_kvcache_fp8", "tree_accept", "tree_metadata",
 ]

@@ -1,0 +1,205 @@
+// Copies of cached data inside the paged KV cache, over every layer, K and V and the row
+// scales in one launch: whole pages (a fork's private copy of a shared page, compaction of
+// a fragmented cache) and single rows (the accepted rows of a tree of drafted tokens,
+// moved to the end of the cached prefix).
+//
+// A copy moves `unit` bytes (a page, or one token's row of all kv heads) from unit src[i]
+// to unit dst[i] of every plane (layer x {K, V}, and their scales). Copies are applied in
+// order i = 0, 1, ..., each seeing what the earlier ones wrote, whatever the indices
+// repeat: a thread owns one 16-byte column of the unit and makes all copies of its column
+// itself, so no other thread ever touches those bytes and program order is the only order
+// needed. Eight copies are in flight per thread (loads first, then stores); when a copy of
+// the eight reads what an earlier one of them writes, the eight are made one at a time.
+//
+// Bound: memory, 2 x unit bytes a copy. The columns of a whole cache (28 layers of 32 KB
+// pages: 114688) with eight 16-byte loads each keep 14 MB in flight, enough to cover the
+// latency of HBM; rows take one group of copies per sequence, groups side by side.
+#include "mkv_common.cuh"
+
+namespace mkv {
+namespace {
+
+constexpr int kCopyThreads = 128;
+constexpr int kInFlight = 8;
+
+struct CopyParams {
+  uint8_t* base[2];      // K and V of layer 0
+  uint8_t* sbase[2];     // their row scales, or null
+  int64_t plane_stride;  // bytes from layer to layer
+  int64_t splane_stride;
+  int64_t unit;          // bytes of a unit of K or V
+  int64_t sunit;         // and of its scales (0: none)
+  int svec;              // column width of the scales, 16 or 4 bytes (K and V: 16)
+  int64_t num_units;
+  int num_layers;
+  const void* src;
+  const void* dst;
+  int i64;
+  int num_copies;        // of a group
+  int num_groups;
+  int32_t* invalid_count;
+};
+
+__device__ __forceinline__ int64_t cp_index(const CopyParams& c, const void* p, int64_t i) {
+  return c.i64 ? __ldg(reinterpret_cast<const int64_t*>(p) + i)
+               : (int64_t)__ldg(reinterpret_cast<const int32_t*>(p) + i);
+}
+
+// Loads and stores in program order (volatile, with a memory clobber): a thread may read
+// what it has written.
+__device__ __forceinline__ uint4 cp_load(const uint8_t* p, uint4) {
+  uint4 r;
+  asm volatile("ld.global.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p) : "memory");
+  return r;
+}
+__device__ __forceinline__ uint32_t cp_load(const uint8_t* p, uint32_t) {
+  uint32_t r;
+  asm volatile("ld.global.u32 %0, [%1];" : "=r"(r) : "l"(p) : "memory");
+  return r;
+}
+__device__ __forceinline__ void cp_store(uint8_t* p, uint4 v) { st_v4(p, v); }
+__device__ __forceinline__ void cp_store(uint8_t* p, uint32_t v) {
+  asm volatile("st.global.u32 [%0], %1;" ::"l"(p), "r"(v) : "memory");
+}
+
+// All copies of one column of a group: p points at its bytes in unit 0, T is its type.
+// A negative entry is no copy; one past the cache is skipped.
+template <typename T>
+__device__ __forceinline__ void copy_column(const CopyParams& c, uint8_t* p, int64_t unit, int64_t first) {
+  for (int i0 = 0; i0 < c.num_copies; i0 += kInFlight) {
+    int64_t s[kInFlight], d[kInFlight];
+    bool chained = false;
+#pragma unroll
+    for (int u = 0; u < kInFlight; ++u) {
+      s[u] = d[u] = -1;
+      if (i0 + u < c.num_copies) {
+        s[u] = cp_index(c, c.src, first + i0 + u);
+        d[u] = cp_index(c, c.dst, first + i0 + u);
+        if (s[u] < 0 || d[u] < 0 || s[u] >= c.num_units || d[u] >= c.num_units) s[u] = d[u] = -1;
+      }
+#pragma unroll
+      for (int w = 0; w < u; ++w) chained |= s[u] >= 0 && s[u] == d[w];
+    }
+    T x[kInFlight];
+    if (!chained) {
+#pragma unroll
+      for (int u = 0; u < kInFlight; ++u)
+        if (s[u] >= 0) x[u] = cp_load(p + s[u] * unit, T());
+#pragma unroll
+      for (int u = 0; u < kInFlight; ++u)
+        if (s[u] >= 0) cp_store(p + d[u] * unit, x[u]);
+    } else {
+#pragma unroll
+      for (int u = 0; u < kInFlight; ++u)
+        if (s[u] >= 0) cp_store(p + d[u] * unit, cp_load(p + s[u] * unit, T()));
+    }
+  }
+}
+
+__global__ void __launch_bounds__(kCopyThreads) copy_units_kernel(const CopyParams c) {
+  const int64_t cols = c.unit / 16, scols = c.sunit ? c.sunit / c.svec : 0;
+  const int64_t planes = 2 * c.num_layers;
+  const int64_t at = (int64_t)blockIdx.x * kCopyThreads + threadIdx.x;
+  for (int g = blockIdx.y; g < c.num_groups; g += gridDim.y) {
+    const int64_t first = (int64_t)g * c.num_copies;
+    if (at < planes * cols) {
+      const int64_t plane = at / cols, col = at - plane * cols;
+      const int64_t layer = plane >> 1;
+      copy_column<uint4>(c, c.base[plane & 1] + layer * c.plane_stride + col * 16, c.unit, first);
+    } else if (at < planes * (cols + scols)) {
+      const int64_t a = at - planes * cols;
+      const int64_t plane = a / scols, col = a - plane * scols;
+      uint8_t* p = c.sbase[plane & 1] + (plane >> 1) * c.splane_stride + col * c.svec;
+      if (c.svec == 16) copy_column<uint4>(c, p, c.sunit, first);
+      else copy_column<uint32_t>(c, p, c.sunit, first);
+    }
+    if (c.invalid_count != nullptr && blockIdx.x == 0) {
+      int bad = 0;
+      for (int i = threadIdx.x; i < c.num_copies; i += kCopyThreads) {
+        const int64_t s = cp_index(c, c.src, first + i), d = cp_index(c, c.dst, first + i);
+        bad += s >= 0 && d >= 0 && (s >= c.num_units || d >= c.num_units);
+      }
+      if (bad) atomicAdd(c.invalid_count, bad);
+    }
+  }
+}
+
+int copy_units(const char* fn, void* k_cache, void* v_cache, int32_t cache_dtype, int32_t num_layers,
+               int64_t layer_stride, int64_t num_blocks, int32_t block_size, int32_t num_kv_heads,
+               int32_t head_dim, float* k_scales, float* v_scales, int64_t scale_layer_stride,
+               const void* src, const void* dst, int32_t index_type, int32_t num_groups,
+               int64_t num_copies, bool pages, int32_t* invalid_count, void* stream) {
+  if (num_layers < 0 || num_blocks < 0 || block_size <= 0 || num_kv_heads <= 0 || head_dim <= 0 ||
+      num_groups < 0 || num_copies < 0 || num_copies > 0x7fffffff - kInFlight)
+    return set_error(MKV_ERR_INVALID_ARGUMENT, "%s: bad sizes", fn);
+  const int bytes = cache_dtype == MKV_DTYPE_INT8 ? 1 : dtype_bytes(cache_dtype);
+  if (bytes == 0) return set_error(MKV_ERR_UNSUPPORTED, "%s: unsupported cache dtype %d", fn, cache_dtype);
+  if (index_type != MKV_INDEX_I32 && index_type != MKV_INDEX_I64)
+    return set_error(MKV_ERR_INVALID_ARGUMENT, "%s: index_type must be MKV_INDEX_I32 or MKV_INDEX_I64", fn);
+  if ((k_scales == nullptr) != (v_scales == nullptr))
+    return set_error(MKV_ERR_INVALID_ARGUMENT, "%s: k_scales and v_scales must both be given or both be NULL", fn);
+  const int64_t row = (int64_t)num_kv_heads * head_dim * bytes;
+  if (row % 16 != 0)
+    return set_error(MKV_ERR_UNSUPPORTED, "%s: a token's row of %lld bytes is not a multiple of 16", fn,
+                     (long long)row);
+  if (num_copies == 0 || num_groups == 0 || num_layers == 0 || num_blocks == 0) return MKV_OK;
+  if (!k_cache || !v_cache || !src || !dst)
+    return set_error(MKV_ERR_INVALID_ARGUMENT, "%s: null pointer argument", fn);
+  if (((uintptr_t)k_cache | (uintptr_t)v_cache | (uint64_t)(layer_stride * bytes)) & 15)
+    return set_error(MKV_ERR_INVALID_ARGUMENT, "%s: caches and layers must be 16-byte aligned", fn);
+  if (((uintptr_t)k_scales | (uintptr_t)v_scales) & 3)
+    return set_error(MKV_ERR_INVALID_ARGUMENT, "%s: scales must be 4-byte aligned", fn);
+  CopyParams c;
+  c.base[0] = (uint8_t*)k_cache;
+  c.base[1] = (uint8_t*)v_cache;
+  c.sbase[0] = (uint8_t*)k_scales;
+  c.sbase[1] = (uint8_t*)v_scales;
+  c.plane_stride = layer_stride * bytes;
+  c.splane_stride = scale_layer_stride * 4;
+  const int64_t rows = pages ? block_size : 1;
+  c.unit = row * rows;
+  c.sunit = k_scales ? rows * num_kv_heads * 4 : 0;
+  c.svec = (((uintptr_t)k_scales | (uintptr_t)v_scales | (uint64_t)c.sunit | (uint64_t)c.splane_stride) & 15) ? 4 : 16;
+  c.num_units = pages ? num_blocks : num_blocks * block_size;
+  c.num_layers = num_layers;
+  c.src = src;
+  c.dst = dst;
+  c.i64 = index_type == MKV_INDEX_I64;
+  c.num_copies = (int)num_copies;
+  c.num_groups = num_groups;
+  c.invalid_count = invalid_count;
+  const int64_t columns = 2 * (int64_t)num_layers * (c.unit / 16 + (c.sunit ? c.sunit / c.svec : 0));
+  const int64_t ctas = (columns + kCopyThreads - 1) / kCopyThreads;
+  if (ctas > 0x7fffffff) return set_error(MKV_ERR_INVALID_ARGUMENT, "%s: bad sizes", fn);
+  const dim3 grid((unsigned)ctas, (unsigned)(num_groups < 65535 ? num_groups : 65535));
+  copy_units_kernel<<<grid, kCopyThreads, 0, (cudaStream_t)stream>>>(c);
+  return cuda_status(cudaGetLastError(), "copy_units launch");
+}
+
+}  // namespace
+}  // namespace mkv
+
+using namespace mkv;
+
+extern "C" int mkv_copy_kv_pages(void* k_cache, void* v_cache, int32_t cache_dtype, int32_t num_layers,
+                                 int64_t layer_stride, int64_t num_blocks, int32_t block_size,
+                                 int32_t num_kv_heads, int32_t head_dim, float* k_scales, float* v_scales,
+                                 int64_t scale_layer_stride, const void* src_pages, const void* dst_pages,
+                                 int32_t index_type, int64_t num_pairs, int32_t* invalid_count, void* stream) {
+  clear_error();
+  return copy_units("mkv_copy_kv_pages", k_cache, v_cache, cache_dtype, num_layers, layer_stride, num_blocks,
+                    block_size, num_kv_heads, head_dim, k_scales, v_scales, scale_layer_stride, src_pages,
+                    dst_pages, index_type, 1, num_pairs, true, invalid_count, stream);
+}
+
+extern "C" int mkv_move_kv_rows(void* k_cache, void* v_cache, int32_t cache_dtype, int32_t num_layers,
+                                int64_t layer_stride, int64_t num_blocks, int32_t block_size,
+                                int32_t num_kv_heads, int32_t head_dim, float* k_scales, float* v_scales,
+                                int64_t scale_layer_stride, const void* src_slots, const void* dst_slots,
+                                int32_t index_type, int32_t num_groups, int32_t moves_per_group,
+                                int32_t* invalid_count, void* stream) {
+  clear_error();
+  return copy_units("mkv_move_kv_rows", k_cache, v_cache, cache_dtype, num_layers, layer_stride, num_blocks,
+                    block_size, num_kv_heads, head_dim, k_scales, v_scales, scale_layer_stride, src_slots,
+                    dst_slots, index_type, num_groups, moves_per_group, false, invalid_count, stream);
+}

@@ -1,0 +1,230 @@
+// Shared parts of the attention for trees of drafted tokens over the paged cache:
+// parameters, the device-side work schedule, and which cached tokens a row sees.
+#pragma once
+
+#include "mkv_common.cuh"
+
+namespace mkv {
+namespace tree {
+
+struct Params {
+  const void* q;
+  int64_t q_st, q_sh;  // elements
+  const uint8_t* k_cache;
+  const uint8_t* v_cache;
+  int64_t num_blocks;
+  int block_size;
+  const void* bt;
+  int64_t bt_sb;
+  int max_blocks, bt_i64;
+  const void* ctx;
+  const void* cu;
+  int ctx_i64, cu_i64;
+  const uint64_t* mask;  // (total_q, mask_words), row stride in words
+  int64_t mask_st;
+  int mask_words;
+  int num_seqs, num_heads, num_kv_heads, head_dim, group;
+  int64_t total_q;
+  float qk_scale_log2;
+  const float* k_scale;   // per-tensor scales of e4m3 pages, or null
+  const float* v_scale;
+  const float* k_scales;  // per-(page, row, kv head) scales of 8-bit pages, or null
+  const float* v_scales;
+  void* out;
+  int64_t o_st, o_sh;  // elements
+  // split units: partial sums (2 slots per CTA) and one descriptor per CTA
+  float* part_acc;  // [slot][row][head_dim], relative to the row's partial maximum
+  float2* part_ml;  // [slot][row] = (maximum in the exp2 domain, sum)
+  int4* desc;
+};
+
+__device__ __forceinline__ int64_t ld_idx(const void* p, int i64, int64_t i) {
+  return i64 ? __ldg(reinterpret_cast<const int64_t*>(p) + i)
+             : (int64_t)__ldg(reinterpret_cast<const int32_t*>(p) + i);
+}
+
+// A sequence of the batch: query rows [q0, q0 + nodes), cached tokens [0, len), the last
+// `nodes` of them the tree's own (from `prefix` on).
+struct Seq {
+  int64_t q0;
+  int nodes, len, prefix;
+};
+__device__ __forceinline__ Seq load_seq(const Params& p, int b) {
+  Seq s;
+  int64_t a = ld_idx(p.cu, p.cu_i64, b), e = ld_idx(p.cu, p.cu_i64, b + 1);
+  a = min(max(a, (int64_t)0), p.total_q);
+  e = min(max(e, (int64_t)0), p.total_q);
+  s.q0 = a;
+  s.nodes = e > a ? (int)(e - a) : 0;
+  const int64_t ctx = ld_idx(p.ctx, p.ctx_i64, b);
+  const int64_t cap = (int64_t)p.max_blocks * p.block_size;  // at most 2^31 - 1 (checked on the host)
+  s.len = (int)max(min(ctx, cap), (int64_t)0);
+  s.prefix = (int)max(min(ctx - s.nodes, (int64_t)s.len), (int64_t)0);
+  return s;
+}
+
+// Page of logical block blk of sequence b, or -1 (entry -1 or outside the cache).
+__device__ __forceinline__ int64_t load_page(const Params& p, int b, int blk) {
+  const int64_t page = ld_idx(p.bt, p.bt_i64, (int64_t)b * p.bt_sb + blk);
+  return (page >= 0 && page < p.num_blocks) ? page : -1;
+}
+
+// Visibility of the 32 tokens t0 .. t0 + 31 for one query row (bit i: token t0 + i): all of
+// the prefix, the tree's nodes by the row's mask, nothing from len on.
+__device__ __forceinline__ uint32_t visible32(const Seq& s, const uint64_t* mask_row, int mask_words, int t0) {
+  const int in = s.len - t0;  // tokens that exist
+  if (in <= 0) return 0u;
+  uint32_t v = in >= 32 ? 0xffffffffu : (1u << in) - 1u;
+  const int j0 = t0 - s.prefix;  // node of bit 0
+  if (j0 <= -32) return v;
+  const int first = j0 < 0 ? 0 : j0;
+  uint64_t bits = 0;
+  if ((first >> 6) < mask_words) bits = __ldg(mask_row + (first >> 6)) >> (first & 63);
+  if ((first & 63) > 32 && (first >> 6) + 1 < mask_words)
+    bits |= __ldg(mask_row + (first >> 6) + 1) << (64 - (first & 63));
+  uint32_t t = (uint32_t)bits;
+  if (j0 < 0) t = (t << -j0) | ((1u << -j0) - 1u);
+  return v & t;
+}
+
+// ---------------------------------------------------------------- work schedule
+// Work items are (sequence, kv head, tile of RT query rows, tile of KT tokens), in this
+// order; a unit is a run of all token tiles of one row tile. CTA c of n takes items
+// [c W / n, (c + 1) W / n): equal work whatever the lengths, known on the device alone. A
+// unit that ends inside a CTA's share is written there whole; the parts of a unit that
+// crosses shares go to partial slots (2 c + 1: the part that starts a unit, 2 c: any later
+// one) and are joined by the combine kernel, which takes its orders from desc[c]: the
+// first CTA that continues a unit names the unit's row tile and the number of its parts.
+struct Unit {
+  int b, kvh, mt;     // sequence, kv head, row tile
+  int k0, k1, tiles;  // token tiles taken here, and of the whole unit
+  Seq s;
+};
+
+template <int RT, int KT>
+__device__ __forceinline__ int64_t items_of(const Params& p, const Seq& s, int& mt, int& kt) {
+  mt = (int)(((int64_t)s.nodes * p.group + RT - 1) / RT);
+  kt = max(1, (s.len + KT - 1) / KT);
+  return (int64_t)p.num_kv_heads * mt * kt;
+}
+
+struct Walk {
+  int64_t at, end;  // items of this CTA not yet taken
+  int b;
+  int64_t off;      // `at` within sequence b
+  int mt, kt;       // of sequence b
+  Seq s;
+};
+
+// Finds CTA c's share. Block-collective over NT threads; writes desc[c]. False when the
+// CTA has nothing to do.
+template <int RT, int KT, int NT>
+__device__ bool begin(const Params& p, int c, int n, Walk& w) {
+  __shared__ long long red[NT / 32];
+  __shared__ long long found[2];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  // inclusive scan of one chunk of sequences; returns this thread's inclusive sum, `sum` the chunk's
+  auto scan = [&](long long x, long long& sum) {
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long v = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += v;
+    }
+    __syncthreads();
+    if (lane == 31) red[warp] = x;
+    __syncthreads();
+    sum = 0;
+#pragma unroll
+    for (int i = 0; i < NT / 32; ++i) {
+      if (i < warp) x += red[i];
+      sum += red[i];
+    }
+    return x;
+  };
+  auto items = [&](int b) -> long long {
+    if (b >= p.num_seqs) return 0;
+    int mt, kt;
+    return items_of<RT, KT>(p, load_seq(p, b), mt, kt);
+  };
+  long long total = 0, mine = 0, incl = 0, sum;
+  for (int base = 0; base < p.num_seqs; base += NT) {
+    mine = items(base + tid);
+    incl = scan(mine, sum);
+    total += sum;
+  }
+  if (n > total) n = (int)total;  // every CTA that works has an item
+  if (tid == 0) p.desc[c] = make_int4(0, 0, 0, 0);
+  if (c >= n) return false;
+  const int64_t s0 = (int64_t)c * total / n, s1 = (int64_t)(c + 1) * total / n;
+  long long before = 0;
+  for (int base = 0; base < p.num_seqs; base += NT) {
+    if (p.num_seqs > NT) {  // otherwise the first scan still holds
+      mine = items(base + tid);
+      incl = scan(mine, sum);
+    }
+    const long long i1 = before + incl;
+    if (mine > 0 && i1 - mine <= s0 && s0 < i1) {
+      found[0] = base + tid;
+      found[1] = s0 - (i1 - mine);
+    }
+    before += sum;
+    if (before > s0) break;
+  }
+  __syncthreads();
+  w.at = s0;
+  w.end = s1;
+  w.b = (int)found[0];
+  w.off = found[1];
+  w.s = load_seq(p, w.b);
+  items_of<RT, KT>(p, w.s, w.mt, w.kt);
+  const int64_t unit0 = s0 - w.off % w.kt;  // first item of the unit that s0 lies in
+  if (tid == 0 && unit0 < s0 && (int64_t)(c - 1) * total / n <= unit0) {
+    // this CTA is the first to continue the unit: parts from CTA c - 1 to the one holding its last item
+    const int64_t last = ((unit0 + w.kt) * n + total - 1) / total - 1;
+    const int u = (int)(w.off / w.kt);
+    p.desc[c] = make_int4(w.b, u / w.mt, u % w.mt, (int)(last - c + 2));
+  }
+  return true;
+}
+
+// The next unit, or the part of it that falls into this CTA's share.
+template <int RT, int KT>
+__device__ __forceinline__ bool next(const Params& p, Walk& w, Unit& u) {
+  if (w.at >= w.end) return false;
+  while (w.off >= (int64_t)p.num_kv_heads * w.mt * w.kt) {  // on to the next sequence that has work
+    w.off -= (int64_t)p.num_kv_heads * w.mt * w.kt;
+    w.s = load_seq(p, ++w.b);
+    items_of<RT, KT>(p, w.s, w.mt, w.kt);
+  }
+  const int64_t i = w.off / w.kt;
+  u.b = w.b;
+  u.s = w.s;
+  u.kvh = (int)(i / w.mt);
+  u.mt = (int)(i % w.mt);
+  u.k0 = (int)(w.off % w.kt);
+  u.tiles = w.kt;
+  u.k1 = (int)min((int64_t)w.kt, u.k0 + (w.end - w.at));
+  w.at += u.k1 - u.k0;
+  w.off += u.k1 - u.k0;
+  return true;
+}
+
+// Partial slot of a unit's part, -1 for a whole unit.
+__device__ __forceinline__ int slot_of(const Unit& u, int c) {
+  if (u.k0 == 0 && u.k1 == u.tiles) return -1;
+  return 2 * c + (u.k0 == 0 ? 1 : 0);
+}
+
+// Sum that a part stores for a row whose visible scores were all -inf (0 / 0 where no other
+// part has a finite one), as opposed to a row that saw nothing (0).
+constexpr float kSeenInf = -1.0f;
+
+// ---------------------------------------------------------------- host side
+constexpr int kSplitCtas = 2 * kNumSMs;  // most CTAs that a kernel here is launched with
+struct Workspace {
+  size_t acc, ml, desc, total;  // offsets and size in bytes
+};
+Workspace workspace(int rows, int head_dim);
+
+}  // namespace tree
+}  // namespace mkv

@@ -17,6 +17,11 @@ Reference (heart1128/mini-kvllm, src/myvllm/engine/model_runner.py):
   KV-head sharding    215      each rank holds num_kv_heads // world_size heads, and the
                                matching num_heads // world_size query heads
                                (models/qwen3.py:27-33)
+
+Not in the reference: decode steps over trees of drafted tokens (tree_metadata, tree_accept,
+move_kv_rows around paged_attention_tree) and copies of whole pages (copy_kv_pages), for a
+block manager that forks sequences or compacts the cache. Which pages are shared or free
+stays the block manager's to know.
 """
 from __future__ import annotations
 
@@ -24,6 +29,9 @@ from dataclasses import dataclass
 from typing import Iterable, Optional, Sequence
 
 import torch
+
+from .. import _lib
+from ..layers.attention import _INDEX, _DTYPES, _on_device, _require_cuda, _stream
 
 PER_TOKEN_HEAD = ("fp8_per_token_head", "int8_per_token_head")
 QUANTIZED = ("fp8_per_tensor",) + PER_TOKEN_HEAD
@@ -197,6 +205,175 @@ class DecodeMetadataBuilder:
         self._lib_mod.check("mkv_decode_metadata", st)
         return DecodeMetadata(slot_mapping=self._slots[:B], context_lens=self._lens[:B],
                               block_tables=self._packed[B:B + B * W].view(B, W))
+
+
+# ------------------------------------------------------------------ trees of drafted tokens
+@dataclass
+class TreeMetadata:
+    slot_mapping: torch.Tensor   # (total_q,) int64
+    context_lens: torch.Tensor   # (B,) int64, the drafted nodes included
+    positions: torch.Tensor      # (total_q,) int64
+    tree_mask: torch.Tensor      # (total_q, words) int64
+
+
+@dataclass
+class TreeAcceptance:
+    num_accepted: torch.Tensor   # (B,) int32
+    accepted_nodes: torch.Tensor  # (B, max_path) int32, -1 padded
+    tokens: torch.Tensor         # (B, max_path) int64, -1 padded
+    context_lens: torch.Tensor   # (B,) int64, cached tokens to keep
+    src_slots: torch.Tensor      # (B, max_path) int64, -1: no move
+    dst_slots: torch.Tensor      # (B, max_path) int64
+
+
+def _indices(fn: str, what: str, t: torch.Tensor, dim: int) -> torch.Tensor:
+    if t.dtype not in _INDEX or t.dim() != dim:
+        raise ValueError(f"{fn}: {what} must be an int32 or int64 tensor of {dim} dimension(s), got "
+                         f"{t.dtype} {tuple(t.shape)}")
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def _tree_args(fn: str, parents, cu_seqlens_q, prefix_lens, block_tables, block_size):
+    """(checked tensors, the argument list that the tree entry points share)"""
+    parents = _indices(fn, "parents", parents, 1)
+    cu = _indices(fn, "cu_seqlens_q", cu_seqlens_q, 1)
+    prefix = _indices(fn, "prefix_lens", prefix_lens, 1)
+    if block_tables.dtype not in _INDEX or block_tables.dim() != 2:
+        raise ValueError(f"{fn}: block_tables must be a two-dimensional int32 or int64 tensor")
+    if block_tables.stride(1) != 1:
+        block_tables = block_tables.contiguous()
+    B = prefix.numel()
+    if cu.numel() != B + 1 or block_tables.shape[0] < B:
+        raise ValueError(f"{fn}: cu_seqlens_q/block_tables do not match {B} sequences")
+    if block_size <= 0:
+        raise ValueError(f"{fn}: block_size must be positive")
+    args = (parents.data_ptr(), _INDEX[parents.dtype], cu.data_ptr(), _INDEX[cu.dtype],
+            prefix.data_ptr(), _INDEX[prefix.dtype], block_tables.data_ptr(),
+            _INDEX[block_tables.dtype], block_tables.stride(0), block_tables.shape[1], block_size, B,
+            parents.numel())
+    return (parents, cu, prefix, block_tables), args
+
+
+def tree_metadata(parents: torch.Tensor, cu_seqlens_q: torch.Tensor, prefix_lens: torch.Tensor,
+                  block_tables: torch.Tensor, block_size: int, max_nodes: int) -> TreeMetadata:
+    """Metadata of a decode step over trees of drafted tokens, in one kernel. parents
+    (total_q,) holds each node's parent within its own tree (a lower index, -1 for a root),
+    sequence b's nodes being rows [cu_seqlens_q[b], cu_seqlens_q[b+1]); prefix_lens[b] tokens
+    are cached before them. Node i is cached at position prefix_lens[b] + i
+    (slot_mapping, -1 without a page), sits at position prefix_lens[b] + its depth
+    (positions) and sees itself and its ancestors (tree_mask). max_nodes bounds every tree
+    (at most 1024). Rows of no sequence get slot -1, which the append skips."""
+    fn = "tree_metadata"
+    if not 1 <= max_nodes <= 1024:
+        raise ValueError(f"{fn}: max_nodes must be 1 to 1024 (got {max_nodes})")
+    dev = _require_cuda(fn, parents, cu_seqlens_q, prefix_lens, block_tables)
+    keep, args = _tree_args(fn, parents, cu_seqlens_q, prefix_lens, block_tables, block_size)
+    B, total, words = args[-2], args[-1], (max_nodes + 63) // 64
+    slots = torch.empty(total, dtype=torch.int64, device=dev)
+    lens = torch.empty(B, dtype=torch.int64, device=dev)
+    positions = torch.empty(total, dtype=torch.int64, device=dev)
+    mask = torch.empty(total, words, dtype=torch.int64, device=dev)
+    with _on_device(dev):
+        st = _lib.load().mkv_tree_metadata(*args, words, slots.data_ptr(), lens.data_ptr(),
+                                           positions.data_ptr(), mask.data_ptr(), None, _stream(dev))
+    _lib.check(fn, st)
+    return TreeMetadata(slots, lens, positions, mask)
+
+
+def tree_accept(draft_tokens: torch.Tensor, target_tokens: torch.Tensor, parents: torch.Tensor,
+                cu_seqlens_q: torch.Tensor, prefix_lens: torch.Tensor, block_tables: torch.Tensor,
+                block_size: int, max_path: int) -> TreeAcceptance:
+    """The path of each tree that the target model agrees with: from node 0, on to the
+    lowest-numbered child whose draft token is the target token of the node before it
+    (target_tokens[row], e.g. the argmax or the sample of the row's logits), at most max_path
+    nodes. Returns the path, its target tokens (the step's new tokens), the number of cached
+    tokens to keep, and the moves that bring the accepted rows there (move_kv_rows). The
+    other arguments as for tree_metadata."""
+    fn = "tree_accept"
+    dev = _require_cuda(fn, draft_tokens, target_tokens, parents, cu_seqlens_q, prefix_lens, block_tables)
+    draft, target = _indices(fn, "draft_tokens", draft_tokens, 1), _indices(fn, "target_tokens", target_tokens, 1)
+    keep, args = _tree_args(fn, parents, cu_seqlens_q, prefix_lens, block_tables, block_size)
+    B, total = args[-2], args[-1]
+    if draft.numel() != total or target.numel() != total or draft.dtype != target.dtype:
+        raise ValueError(f"{fn}: draft_tokens and target_tokens must be {total} tokens each, of one dtype")
+    if max_path < 1:
+        raise ValueError(f"{fn}: max_path must be at least 1 (got {max_path})")
+    # (B, max_path) rows of int64, then of int32, and the two counts, in one allocation each
+    wide = torch.empty(B * (3 * max_path + 1), dtype=torch.int64, device=dev)
+    narrow = torch.empty(B * (max_path + 1), dtype=torch.int32, device=dev)
+    n = B * max_path
+    tokens, src, dst, lens = wide[:n], wide[n:2 * n], wide[2 * n:3 * n], wide[3 * n:]
+    nodes, count = narrow[:n], narrow[n:]
+    with _on_device(dev):
+        st = _lib.load().mkv_tree_accept(
+            draft.data_ptr(), target.data_ptr(), _INDEX[draft.dtype], *args, max_path, count.data_ptr(),
+            nodes.data_ptr(), tokens.data_ptr(), lens.data_ptr(), src.data_ptr(), dst.data_ptr(),
+            _stream(dev))
+    _lib.check(fn, st)
+    shape = (B, max_path)
+    return TreeAcceptance(count, nodes.view(shape), tokens.view(shape), lens, src.view(shape), dst.view(shape))
+
+
+# ------------------------------------------------------------------ copies inside the cache
+def _cache_args(fn: str, cache: KVCache):
+    kv = cache.kv
+    if kv.dim() != 6 or kv.shape[0] != 2 or not kv.is_contiguous():
+        raise ValueError(f"{fn}: the cache must be one contiguous (2, L, NB, BS, KVH, D) tensor")
+    if kv.dtype not in _DTYPES:
+        raise ValueError(f"{fn}: unsupported cache dtype {kv.dtype}")
+    _, L, NB, BS, KVH, D = kv.shape
+    ks = vs = None
+    stride = 0
+    if cache.kv_cache_dtype in PER_TOKEN_HEAD:
+        for t in (cache.k_scale, cache.v_scale):
+            if t is None or t.dtype != torch.float32 or t.shape != (L, NB, BS, KVH) or not t.is_contiguous():
+                raise ValueError(f"{fn}: {cache.kv_cache_dtype} needs contiguous float32 scales ({L}, {NB}, {BS}, {KVH})")
+        ks, vs, stride = cache.k_scale.data_ptr(), cache.v_scale.data_ptr(), NB * BS * KVH
+    k = kv.data_ptr()
+    v = k + kv.numel() // 2 * kv.element_size()
+    return (k, v, _DTYPES[kv.dtype], L, NB * BS * KVH * D, NB, BS, KVH, D, ks, vs, stride)
+
+
+def _pairs(fn: str, cache: KVCache, src: torch.Tensor, dst: torch.Tensor, dim: int):
+    tensors = (cache.kv, src, dst)
+    if cache.kv_cache_dtype in PER_TOKEN_HEAD and cache.k_scale is not None and cache.v_scale is not None:
+        tensors += (cache.k_scale, cache.v_scale)
+    dev = _require_cuda(fn, *tensors)
+    src, dst = _indices(fn, "the source", src, dim), _indices(fn, "the destination", dst, dim)
+    if src.shape != dst.shape or src.dtype != dst.dtype:
+        raise ValueError(f"{fn}: source and destination must have one shape and dtype")
+    return dev, src, dst
+
+
+def copy_kv_pages(cache: KVCache, src_pages: torch.Tensor, dst_pages: torch.Tensor) -> None:
+    """Copies page src_pages[i] to page dst_pages[i] of every layer, K and V and the
+    per-(token, head) scales, in one kernel: a forked sequence's own copy of a shared page,
+    or the moves of a compaction. The copies are made in order, so one that reads a page
+    written by an earlier one sees what was written; an entry below 0 is no copy, one past
+    the cache is skipped."""
+    fn = "copy_kv_pages"
+    dev, src, dst = _pairs(fn, cache, src_pages, dst_pages, 1)
+    args = _cache_args(fn, cache)
+    with _on_device(dev):
+        st = _lib.load().mkv_copy_kv_pages(*args, src.data_ptr(), dst.data_ptr(), _INDEX[src.dtype],
+                                           src.numel(), None, _stream(dev))
+    _lib.check(fn, st)
+
+
+def move_kv_rows(cache: KVCache, src_slots: torch.Tensor, dst_slots: torch.Tensor) -> None:
+    """Copies the cached row of slot src_slots[g, i] to slot dst_slots[g, i] in every layer,
+    K and V and the per-(token, head) scales, in one kernel: the accepted rows of a tree,
+    moved to the end of the cached prefix (tree_accept gives the slots). Moves are made in
+    order within a group g (a sequence); the groups run side by side, so what one of them
+    writes no other may read or write. An entry below 0 is no move, one past the cache is
+    skipped."""
+    fn = "move_kv_rows"
+    dev, src, dst = _pairs(fn, cache, src_slots, dst_slots, 2)
+    args = _cache_args(fn, cache)
+    with _on_device(dev):
+        st = _lib.load().mkv_move_kv_rows(*args, src.data_ptr(), dst.data_ptr(), _INDEX[src.dtype],
+                                          src.shape[0], src.shape[1], None, _stream(dev))
+    _lib.check(fn, st)
 
 
 def kv_head_shard(num_heads: int, num_kv_heads: int, rank: int, world_size: int):

@@ -17,7 +17,8 @@ The functions keep the reference's names, argument order and meaning
                           cu_seqlens_q, positions, scale, num_heads, num_kv_heads,
                           head_dim, block_size)        # paged_attention_prefill_triton :852
 
-with kv_cache_dtype "fp8_per_tensor" (scales of shape (1,)), "fp8_per_token_head" and
+and, without a counterpart there, paged_attention_tree for decode steps over trees of
+drafted tokens, with kv_cache_dtype "fp8_per_tensor" (scales of shape (1,)), "fp8_per_token_head" and
 "int8_per_token_head" (scales of shape (num_blocks, block_size, num_kv_heads)).
 
 and `Attention` keeps the module contract of attention.py:1617-1807 (cache tensors and
@@ -549,6 +550,101 @@ def flash_attention_prefill(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     return out
 
 
+# ---------------------------------------------------------------------------------- trees
+def paged_attention_tree(query: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                         block_tables: torch.Tensor, context_lens: torch.Tensor,
+                         cu_seqlens_q: torch.Tensor, tree_mask: torch.Tensor, scale: float,
+                         num_heads: int, num_kv_heads: int, head_dim: int, block_size: int,
+                         k_scale: torch.Tensor | None = None, v_scale: torch.Tensor | None = None,
+                         kv_cache_dtype: str = "auto", out: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of trees of drafted tokens over the paged cache: query (total_q, num_heads,
+    head_dim) holds every sequence's drafted nodes (sequence b owns rows
+    [cu_seqlens_q[b], cu_seqlens_q[b+1])), whose K/V have been appended as the last tokens
+    of its context_lens[b] cached ones. A row sees every token before the sequence's nodes,
+    and node j when bit j % 64 of its word tree_mask[row, j // 64] (int64, as tree_metadata
+    makes it) is set. Returns (total_q, num_heads, head_dim) in the query dtype; a row that
+    sees nothing is 0, and rows of no sequence (a padded batch's) are not written: with
+    `out` given they keep what it held. Caches and scales as for paged_attention_prefill.
+    Not in the reference, which decodes one token per sequence and step."""
+    fn = "paged_attention_tree"
+    if query.dim() != 3 or query.shape[1] != num_heads or query.shape[2] != head_dim:
+        raise ValueError(f"{fn}: query must be (total_q, {num_heads}, {head_dim}), got {tuple(query.shape)}")
+    if query.dtype not in _FLOAT_IO:
+        raise ValueError(f"{fn}: unsupported query dtype {query.dtype}")
+    tensors = [query, k_cache, v_cache, block_tables, context_lens, cu_seqlens_q, tree_mask]
+    quant = kv_cache_dtype != "auto"
+    if quant:
+        if kv_cache_dtype not in ("fp8_per_tensor",) + _PER_TOKEN_HEAD:
+            raise NotImplementedError(f"{fn}: kv_cache_dtype {kv_cache_dtype!r} is not implemented")
+        if k_scale is None or v_scale is None:
+            raise ValueError(f"{fn}: {kv_cache_dtype} needs k_scale and v_scale")
+        tensors += [k_scale, v_scale]
+    if out is not None:
+        if out.shape != query.shape or out.dtype != query.dtype or (out.numel() and out.stride(-1) != 1):
+            raise ValueError(f"{fn}: out must have the query's shape and dtype, and contiguous rows")
+        tensors.append(out)
+    dev = _require_cuda(fn, *tensors)
+    total_q, num_seqs = query.shape[0], context_lens.numel()
+    if tree_mask.dtype != torch.int64 or tree_mask.dim() != 2 or tree_mask.shape[0] != total_q or \
+            tree_mask.shape[1] < 1:
+        raise ValueError(f"{fn}: tree_mask must be int64 ({total_q}, words), got {tree_mask.dtype} "
+                         f"{tuple(tree_mask.shape)}")
+    if block_tables.dim() != 2 or block_tables.dtype not in _INDEX:
+        raise ValueError(f"{fn}: block_tables must be a two-dimensional int32 or int64 tensor")
+    lens = _index_tensor(context_lens.reshape(-1), fn, "context_lens")
+    cu = _index_tensor(cu_seqlens_q.reshape(-1), fn, "cu_seqlens_q")
+    if cu.numel() != num_seqs + 1 or block_tables.shape[0] < num_seqs:
+        raise ValueError(f"{fn}: cu_seqlens_q/block_tables do not match {num_seqs} sequences")
+    num_blocks = _check_cache(fn, k_cache, v_cache, block_size, num_kv_heads, head_dim)
+    kp = vp = kps = vps = None
+    if not quant:
+        if k_cache.dtype != query.dtype:
+            raise ValueError(f"{fn}: cache dtype {k_cache.dtype} must equal the query dtype {query.dtype}")
+        cache_code = _DTYPES[k_cache.dtype]
+    elif kv_cache_dtype == "fp8_per_tensor":
+        if k_cache.dtype not in (torch.float8_e4m3fn, torch.uint8):
+            raise ValueError(f"{fn}: fp8_per_tensor needs float8_e4m3fn caches (got {k_cache.dtype})")
+        if k_scale.dtype != torch.float32 or v_scale.dtype != torch.float32 or \
+                k_scale.numel() < 1 or v_scale.numel() < 1:
+            raise ValueError(f"{fn}: k_scale/v_scale must be float32 tensors with one element")
+        kp, vp = k_scale.data_ptr(), v_scale.data_ptr()
+        cache_code = _lib.DTYPE_FP8_E4M3
+    else:
+        want = torch.int8 if kv_cache_dtype.startswith("int8") else torch.float8_e4m3fn
+        if k_cache.dtype != want:
+            raise ValueError(f"{fn}: {kv_cache_dtype} needs {want} caches (got {k_cache.dtype})")
+        _check_row_scales(fn, k_scale, v_scale, num_blocks, block_size, num_kv_heads)
+        kps, vps = k_scale.data_ptr(), v_scale.data_ptr()
+        cache_code = _DTYPES[want]
+    output = out if out is not None else torch.empty(query.shape, dtype=query.dtype, device=dev)
+    if total_q == 0 or num_seqs == 0:
+        return output
+    if query.stride(-1) != 1:
+        query = query.contiguous()
+    if block_tables.stride(-1) != 1:
+        block_tables = block_tables.contiguous()
+    if tree_mask.stride(-1) != 1:
+        tree_mask = tree_mask.contiguous()
+    lib = _lib.load()
+    dt = _DTYPES[query.dtype]
+    ws_n = lib.mkv_paged_tree_workspace_bytes(num_seqs, total_q, num_heads, num_kv_heads, head_dim, dt,
+                                              cache_code)
+    # from the caching allocator at each call: calls on other streams, and captured graphs,
+    # never share a workspace
+    ws = torch.empty(ws_n, dtype=torch.uint8, device=dev)
+    with _on_device(dev):
+        st = lib.mkv_paged_tree_attention(
+            query.data_ptr(), query.stride(0), query.stride(1), dt, k_cache.data_ptr(),
+            v_cache.data_ptr(), cache_code, kp, vp, kps, vps, num_blocks, block_size,
+            block_tables.data_ptr(), _INDEX[block_tables.dtype], block_tables.stride(0),
+            block_tables.shape[1], lens.data_ptr(), _INDEX[lens.dtype], cu.data_ptr(),
+            _INDEX[cu.dtype], tree_mask.data_ptr(), tree_mask.stride(0), tree_mask.shape[1], num_seqs,
+            total_q, num_heads, num_kv_heads, head_dim, float(scale), output.data_ptr(),
+            output.stride(0), output.stride(1), ws.data_ptr(), ws_n, _stream(dev))
+    _lib.check(fn, st)
+    return output
+
+
 # ---------------------------------------------------------------------------------- module
 class Attention(nn.Module):
     """Attention layer with a paged KV cache (reference attention.py:1617-1807).
@@ -560,7 +656,8 @@ class Attention(nn.Module):
     per-(token, head) modes).
     `forward` appends the step's K/V at context.slot_mapping and, for a decode batch,
     returns (batch, num_heads * head_dim); a prefill, chunked-prefill or mixed batch
-    attends through the paged cache (paged_attention_prefill for its prefill rows)."""
+    attends through the paged cache (paged_attention_prefill for its prefill rows). A step
+    whose context holds a tree_mask attends with paged_attention_tree."""
 
     def __init__(self, num_heads: int, head_dim: int, scale: float = 1.0,
                  num_kv_heads: int | None = None, block_size: int = 16):
@@ -597,6 +694,14 @@ class Attention(nn.Module):
             else:
                 store_kvcache(k, v, k_cache, v_cache, context.slot_mapping, self.block_size)
         scale = self.scale / (self.head_dim ** 0.5)
+        if context.tree_mask is not None:  # a step over trees of drafted tokens
+            if context.cu_seqlens_q is None or context.context_lens is None or context.block_tables is None:
+                raise ValueError("a tree step requires cu_seqlens_q, context_lens and block_tables")
+            o = paged_attention_tree(
+                q, k_cache, v_cache, context.block_tables, context.context_lens, context.cu_seqlens_q,
+                context.tree_mask, scale, self.num_heads, self.num_kv_heads, self.head_dim,
+                self.block_size, self.k_scale, self.v_scale, mode)
+            return o.reshape(o.shape[0], self.num_heads * self.head_dim)
         if context.is_prefill:
             if getattr(context, "is_full_prefill", False):
                 # every sequence is a whole prompt: attend over the step's own q/k/v, as the

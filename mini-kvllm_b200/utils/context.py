@@ -8,6 +8,8 @@ model runner written against the reference fills it the same way:
   context_lens  (num_seqs,)            int64, tokens visible to each decode query,
                                        including the one being appended
   block_tables  (num_seqs, max_blocks) int32, physical page of each logical block, -1 padded
+and, for a step over trees of drafted tokens (not in the reference),
+  tree_mask     (num_tokens, words)    int64, which nodes of its tree each token sees
 """
 from __future__ import annotations
 
@@ -48,6 +50,7 @@ class Context:
     is_full_prefill: bool = False
     residual_slots: Optional[Any] = None
     residual_lens: Optional[Any] = None
+    tree_mask: Optional[Any] = None
 
 
 def split_mixed_decode_prefill_metadata(cu_seqlens_q, query_lens, is_decode) -> MixedAttentionSplit:
@@ -89,11 +92,13 @@ def reset_context() -> None:
 def set_context(is_prefill, cu_seqlens_q=None, cu_seqlens_k=None, max_seqlen_q=0, max_seqlen_k=0,
                 slot_mapping=None, context_lens=None, block_tables=None, positions=None,
                 query_lens=None, is_decode=None, mixed_attention_split=None,
-                is_full_prefill=False, residual_slots=None, residual_lens=None) -> None:
+                is_full_prefill=False, residual_slots=None, residual_lens=None,
+                tree_mask=None) -> None:
     global _context
     _context = Context(
         is_prefill=is_prefill, cu_seqlens_q=cu_seqlens_q, cu_seqlens_k=cu_seqlens_k,
         max_seqlen_q=max_seqlen_q, max_seqlen_k=max_seqlen_k, slot_mapping=slot_mapping,
         context_lens=context_lens, block_tables=block_tables, positions=positions,
         query_lens=query_lens, is_decode=is_decode, mixed_attention_split=mixed_attention_split,
-        is_full_prefill=is_full_prefill, residual_slots=residual_slots, residual_lens=residual_lens)
+        is_full_prefill=is_full_prefill, residual_slots=residual_slots, residual_lens=residual_lens,
+        tree_mask=tree_mask)

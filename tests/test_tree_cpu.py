@@ -1,0 +1,146 @@
+"""Refusals of the tree and cache-copy entry points, through the C ABI and the wrappers; no
+call here reaches a CUDA API."""
+import pytest
+import torch
+
+from conftest import mkv_module
+
+lib_mod = mkv_module("_lib")
+kv = mkv_module("engine.kv_cache")
+P = 1 << 20  # a pointer that nothing reads
+
+
+def _tree(lib, **kw):
+    a = dict(q=P, qst=1024, qsh=128, qdt=2, k=P, v=P, cdt=2, ks=None, vs=None, kss=None, vss=None, nb=10, bs=16, bt=P,
+             btt=0, btst=8, maxb=8, cl=P, clt=1, cu=P, cut=0, mask=P, mst=1, words=1, B=2, T=9, H=8, KVH=2, D=128,
+             scale=0.1, out=P, ost=1024, osh=128, ws=P, wsb=1 << 40, stream=None)
+    assert set(kw) <= set(a)
+    a.update(kw)
+    return lib.mkv_paged_tree_attention(*a.values())
+
+
+@pytest.mark.parametrize("kw,status,msg", [
+    (dict(H=7), 1, b"multiple of num_kv_heads"),
+    (dict(D=100), 2, b"head_dim"),
+    (dict(D=272), 2, b"head_dim"),
+    (dict(qdt=3), 2, b"query dtype"),
+    (dict(cdt=1), 2, b"cache dtype"),
+    (dict(cdt=3), 1, b"needs k_scale and v_scale"),
+    (dict(cdt=3, ks=P), 1, b"needs k_scale and v_scale"),
+    (dict(cdt=3, ks=P, vs=P, kss=P, vss=P), 1, b"needs k_scale and v_scale"),
+    (dict(cdt=4, ks=P, vs=P), 1, b"INT8"),
+    (dict(ks=P, vs=P), 1, b"unquantised"),
+    (dict(btt=2), 1, b"index types"),
+    (dict(clt=-1), 1, b"index types"),
+    (dict(cut=9), 1, b"index types"),
+    (dict(words=0), 1, b"bad sizes"),
+    (dict(bs=0), 1, b"bad sizes"),
+    (dict(B=-1), 1, b"bad sizes"),
+    (dict(q=None), 1, b"null pointer"),
+    (dict(mask=None), 1, b"null pointer"),
+    (dict(bt=None), 1, b"null pointer"),
+    (dict(k=P + 8), 1, b"16-byte aligned"),
+    (dict(ws=None), 3, b"workspace"),
+    (dict(wsb=1000), 3, b"workspace"),
+    (dict(ws=P + 4), 3, b"workspace"),
+    (dict(maxb=1 << 28), 2, b"2^31 tokens"),
+    (dict(T=1 << 40), 2, b"2^31"),
+])
+def test_attention_refusals(kw, status, msg):
+    lib = lib_mod.load()
+    assert _tree(lib, **kw) == status
+    assert msg in lib.mkv_last_error()
+
+
+def test_nothing_to_do():
+    lib = lib_mod.load()
+    assert _tree(lib, B=0, q=None, out=None, ws=None, wsb=0) == 0
+    assert _tree(lib, T=0, q=None, out=None, ws=None, wsb=0) == 0
+    assert lib.mkv_paged_tree_workspace_bytes(0, 5, 8, 2, 128, 2, 2) == 0
+    assert lib.mkv_paged_tree_workspace_bytes(2, 9, 8, 2, 128, 2, 2) > 0
+    assert lib.mkv_tree_metadata(None, 0, None, 0, None, 0, None, 0, 0, 0, 16, 0, 0, 1, None, None, None, None, None,
+                                 None) == 0
+    assert lib.mkv_copy_kv_pages(None, None, 2, 4, 0, 10, 16, 2, 128, None, None, 0, None, None, 0, 0, None, None) == 0
+    assert lib.mkv_move_kv_rows(None, None, 2, 4, 0, 10, 16, 2, 128, None, None, 0, None, None, 0, 3, 0, None, None) == 0
+
+
+@pytest.mark.parametrize("kw,status,msg", [
+    (dict(pt=7), 1, b"index types"), (dict(words=0), 2, b"mask_words"), (dict(words=17), 2, b"mask_words"),
+    (dict(bs=0), 1, b"bad sizes"), (dict(B=-2), 1, b"bad sizes"), (dict(cu=None), 1, b"null pointer"),
+    (dict(slots=None), 1, b"null output"), (dict(bt=None), 1, b"null pointer")])
+def test_metadata_refusals(kw, status, msg):
+    a = dict(par=P, pt=0, cu=P, ct=0, pre=P, prt=1, bt=P, btt=0, bts=4, maxb=4, bs=16, B=2, T=5, words=1, slots=P, lens=P,
+             pos=P, mask=P, bad=None, stream=None)
+    a.update(kw)
+    lib = lib_mod.load()
+    assert lib.mkv_tree_metadata(*a.values()) == status
+    assert msg in lib.mkv_last_error()
+
+
+@pytest.mark.parametrize("kw,status,msg", [
+    (dict(tt=3), 1, b"token_index_type"), (dict(path=0), 1, b"max_path"), (dict(draft=None), 1, b"null pointer"),
+    (dict(dst=None), 1, b"null pointer"), (dict(T=-1), 1, b"bad sizes")])
+def test_accept_refusals(kw, status, msg):
+    a = dict(draft=P, target=P, tt=1, par=P, pt=0, cu=P, ct=0, pre=P, prt=1, bt=P, btt=0, bts=4, maxb=4, bs=16, B=2, T=5,
+             path=3, count=P, nodes=P, tokens=P, lens=P, src=P, dst=P, stream=None)
+    a.update(kw)
+    lib = lib_mod.load()
+    assert lib.mkv_tree_accept(*a.values()) == status
+    assert msg in lib.mkv_last_error()
+
+
+@pytest.mark.parametrize("kw,status,msg", [
+    (dict(cdt=7), 2, b"cache dtype"), (dict(D=4, KVH=1), 2, b"multiple of 16"), (dict(it=4), 1, b"index_type"),
+    (dict(ks=P), 1, b"both"), (dict(k=P + 8), 1, b"16-byte aligned"), (dict(ls=4), 1, b"16-byte aligned"),
+    (dict(ks=P + 2, vs=P), 1, b"4-byte aligned"), (dict(src=None), 1, b"null pointer"), (dict(NB=-1), 1, b"bad sizes"),
+    (dict(n=1 << 40), 1, b"bad sizes")])
+def test_copy_refusals(kw, status, msg):
+    a = dict(k=P, v=P, cdt=2, L=2, ls=40960, NB=10, BS=16, KVH=2, D=128, ks=None, vs=None, ss=0, src=P, dst=P, it=1, n=3,
+             bad=None, stream=None)
+    a.update(kw)
+    lib = lib_mod.load()
+    assert lib.mkv_copy_kv_pages(*a.values()) == status
+    assert msg in lib.mkv_last_error()
+
+
+def test_wrappers_refuse(attn):
+    q = torch.zeros(3, 8, 128, dtype=torch.bfloat16)
+    c = torch.zeros(8, 16, 2, 128, dtype=torch.bfloat16)
+    i = torch.zeros(1, dtype=torch.int32)
+    bt, cu, mask = torch.zeros(1, 4, dtype=torch.int32), torch.tensor([0, 3]), torch.zeros(3, 1, dtype=torch.int64)
+    args = (c, c, bt, i, cu, mask, 0.1, 8, 2, 128, 16)
+    with pytest.raises(ValueError, match="CUDA"):
+        attn.paged_attention_tree(q, *args)
+    with pytest.raises(ValueError, match="query must be"):
+        attn.paged_attention_tree(q[:, :4], *args)
+    with pytest.raises(ValueError, match="query dtype"):
+        attn.paged_attention_tree(q.double(), *args)
+    with pytest.raises(NotImplementedError, match="kivi"):
+        attn.paged_attention_tree(q, *args, None, None, "kivi_2bit")
+    with pytest.raises(ValueError, match="needs k_scale"):
+        attn.paged_attention_tree(q, *args, None, None, "fp8_per_tensor")
+    with pytest.raises(ValueError, match="out must"):
+        attn.paged_attention_tree(q, *args, out=torch.zeros(3, 8, 128))
+    par = torch.zeros(3, dtype=torch.int32)
+    with pytest.raises(ValueError, match="CUDA"):
+        kv.tree_metadata(par, cu, i, bt, 16, 8)
+    with pytest.raises(ValueError, match="max_nodes"):
+        kv.tree_metadata(par, cu, i, bt, 16, 1025)
+    with pytest.raises(ValueError, match="CUDA"):
+        kv.tree_accept(par.long(), par.long(), par, cu, i, bt, 16, 4)
+    cache = kv.allocate_kv_cache(2, 4, 16, 2, 64, device="cpu")
+    with pytest.raises(ValueError, match="CUDA"):
+        kv.copy_kv_pages(cache, par, par)
+    with pytest.raises(ValueError, match="CUDA"):
+        kv.move_kv_rows(cache, par.view(1, 3), par.view(1, 3))
+
+
+def test_the_oracle_itself():
+    """The plain implementations on an example worked out by hand."""
+    from oracle.tree_oracle import mask_words, tree_accept_ref, tree_metadata_ref
+    parents, cu, tables = [-1, 0, 0, 2, 2], [0, 5], [[7, 4]]
+    slots, lens, positions, visible = tree_metadata_ref(parents, cu, [14], tables, 16, 1)
+    assert slots == [126, 127, 64, 65, 66] and lens == [19] and positions == [14, 15, 15, 16, 16]
+    assert mask_words(visible, 1).tolist() == [[1], [3], [5], [13], [21]]
+    got = tree_accept_ref([9, 5, 6, 8, 8], [6, 1, 8, 2, 3], parents, cu, [14], tables, 16, 4)
+    assert got == ([3], [[0, 2, 3, -1]], [[6, 8, 2, -1]], [17], [[-1, 64, 65, -1]], [[-1, 127, 64, -1]])
