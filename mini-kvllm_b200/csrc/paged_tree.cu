@@ -20,6 +20,7 @@ namespace {
 // Every type and head_dim (a multiple of 16, at most 256): 16 rows x 32 tokens per step in
 // fp32. A warp owns 4 rows; lane = token for the scores, lane = column for the products.
 constexpr int kGRows = 16, kGKT = 32, kGThreads = 128;
+constexpr int kGCtas = 2 * kNumSMs;
 
 template <typename CT> __device__ __forceinline__ float elem_f32(const uint8_t* p, int i) {
   return to_f32(reinterpret_cast<const CT*>(p)[i]);
@@ -35,12 +36,13 @@ __global__ void __launch_bounds__(kGThreads) paged_tree_generic_kernel(const Par
   float* p_sm = v_sm + kGKT * D;       // [warp][32 tokens][4 rows]
   float* ks_sm = p_sm + kGRows * kGKT; // [32]
   __shared__ uint32_t page_ok;
+  __shared__ long long scratch[kBeginWords(kGThreads)];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   constexpr int kVec = 16 / (int)sizeof(CT);
   const bool per_token = p.k_scales != nullptr;
   const float kst = p.k_scale ? __ldg(p.k_scale) : 1.0f, vst = p.v_scale ? __ldg(p.v_scale) : 1.0f;
   Walk w;
-  if (!begin<kGRows, kGKT, kGThreads>(p, blockIdx.x, gridDim.x, w)) return;
+  if (!begin<kGRows, kGKT, kGThreads>(p, blockIdx.x, gridDim.x, scratch, w)) return;
   Unit u;
   while (next<kGRows, kGKT>(p, w, u)) {
     const int rows = min(kGRows, u.s.nodes * p.group - u.mt * kGRows);
@@ -241,7 +243,8 @@ __global__ void __launch_bounds__(32 * kCWarps) paged_tree_combine_kernel(const 
 template <typename QT>
 int launch_combine(const Params& p, int ctas, int rows, cudaStream_t s) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(ctas, ceil_div(rows, kCWarps));
+  const int64_t most = p.total_q * p.group;  // rows that a unit can have
+  cfg.gridDim = dim3(ctas, ceil_div(most < rows ? most : rows, kCWarps));
   cfg.blockDim = dim3(32 * kCWarps);
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
@@ -258,30 +261,35 @@ int launch_generic(const Params& p, cudaStream_t s) {
   const void* f = (const void*)paged_tree_generic_kernel<QT, CT>;
   int st = ensure_dynamic_smem(f, bytes, "paged_tree_generic shared memory");
   if (st != MKV_OK) return st;
-  const int ctas = kSplitCtas;
-  paged_tree_generic_kernel<QT, CT><<<ctas, kGThreads, bytes, s>>>(p);
-  st = cuda_status(cudaGetLastError(), "paged_tree_generic launch");
-  return st == MKV_OK ? launch_combine<QT>(p, ctas, kGRows, s) : st;
+  paged_tree_generic_kernel<QT, CT><<<kGCtas, kGThreads, bytes, s>>>(p);
+  return cuda_status(cudaGetLastError(), "paged_tree_generic launch");
 }
 
+// How a call is run: the kernel, its row tile and its CTAs.
+struct Plan {
+  bool tc;
+  int rows, ctas;
+};
+
 template <typename QT>
-int dispatch(const Params& p, int cache_dtype, cudaStream_t s) {
-  switch (cache_dtype) {
-    case MKV_DTYPE_FP8_E4M3: return launch_generic<QT, fp8>(p, s);
-    case MKV_DTYPE_INT8: return launch_generic<QT, int8_t>(p, s);
-    default: return launch_generic<QT, QT>(p, s);
-  }
+int run(const Params& p, const Plan& plan, int q_dtype, int cache_dtype, cudaStream_t s) {
+  int st;
+  if (plan.tc) st = launch_tc(p, q_dtype, cache_dtype, plan.ctas, s);
+  else if (cache_dtype == MKV_DTYPE_FP8_E4M3) st = launch_generic<QT, fp8>(p, s);
+  else if (cache_dtype == MKV_DTYPE_INT8) st = launch_generic<QT, int8_t>(p, s);
+  else st = launch_generic<QT, QT>(p, s);
+  return st == MKV_OK ? launch_combine<QT>(p, plan.ctas, plan.rows, s) : st;
 }
 
 }  // namespace
 
-Workspace workspace(int rows, int head_dim) {
+Workspace workspace(int ctas, int rows, int head_dim) {
   auto up = [](size_t x) { return (x + 255) / 256 * 256; };
   Workspace w;
   w.acc = 0;
-  w.ml = up((size_t)2 * kSplitCtas * rows * head_dim * 4);
-  w.desc = w.ml + up((size_t)2 * kSplitCtas * rows * 8);
-  w.total = w.desc + up((size_t)kSplitCtas * 16);
+  w.ml = up((size_t)2 * ctas * rows * head_dim * 4);
+  w.desc = w.ml + up((size_t)2 * ctas * rows * 8);
+  w.total = w.desc + up((size_t)ctas * 16);
   return w;
 }
 
@@ -294,7 +302,10 @@ extern "C" size_t mkv_paged_tree_workspace_bytes(int32_t num_seqs, int64_t total
                                                  int32_t num_kv_heads, int32_t head_dim, int32_t q_dtype,
                                                  int32_t cache_dtype) {
   if (num_seqs <= 0 || total_q <= 0 || num_kv_heads <= 0 || num_heads <= 0 || head_dim <= 0) return 0;
-  return tree::workspace(tree::kGRows, head_dim).total;
+  // the larger of the two kernels' (which of them runs depends on the tensors' alignment too)
+  const size_t generic = tree::workspace(tree::kGCtas, tree::kGRows, head_dim).total;
+  const size_t tc = tree::workspace(kNumSMs, tree::kTcRows, head_dim).total;
+  return head_dim == 128 && q_dtype != MKV_DTYPE_F32 && tc > generic ? tc : generic;
 }
 
 extern "C" int mkv_paged_tree_attention(
@@ -381,14 +392,17 @@ extern "C" int mkv_paged_tree_attention(
   p.out = out;
   p.o_st = out_stride_token;
   p.o_sh = out_stride_head;
-  const tree::Workspace w = tree::workspace(tree::kGRows, head_dim);
+  const tree::Plan plan = tree::tc_supported(p, q_dtype, cache_dtype)
+                              ? tree::Plan{true, tree::kTcRows, kNumSMs}
+                              : tree::Plan{false, tree::kGRows, tree::kGCtas};
+  const tree::Workspace w = tree::workspace(plan.ctas, plan.rows, head_dim);
   p.part_acc = (float*)((char*)workspace + w.acc);
   p.part_ml = (float2*)((char*)workspace + w.ml);
   p.desc = (int4*)((char*)workspace + w.desc);
   cudaStream_t s = (cudaStream_t)stream;
   switch (q_dtype) {
-    case MKV_DTYPE_F16: return tree::dispatch<f16>(p, cache_dtype, s);
-    case MKV_DTYPE_BF16: return tree::dispatch<bf16>(p, cache_dtype, s);
-    default: return tree::dispatch<float>(p, cache_dtype, s);
+    case MKV_DTYPE_F16: return tree::run<f16>(p, plan, q_dtype, cache_dtype, s);
+    case MKV_DTYPE_BF16: return tree::run<bf16>(p, plan, q_dtype, cache_dtype, s);
+    default: return tree::run<float>(p, plan, q_dtype, cache_dtype, s);
   }
 }

@@ -116,12 +116,13 @@ struct Walk {
   Seq s;
 };
 
-// Finds CTA c's share. Block-collective over NT threads; writes desc[c]. False when the
-// CTA has nothing to do.
+// Finds CTA c's share. Block-collective over NT threads, with kBeginWords(NT) words of
+// shared memory that are free again after the caller's next barrier; writes desc[c]. False
+// when the CTA has nothing to do.
+constexpr int kBeginWords(int nt) { return nt / 32 + 2; }
 template <int RT, int KT, int NT>
-__device__ bool begin(const Params& p, int c, int n, Walk& w) {
-  __shared__ long long red[NT / 32];
-  __shared__ long long found[2];
+__device__ bool begin(const Params& p, int c, int n, long long* red, Walk& w) {
+  long long* found = red + NT / 32;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   // inclusive scan of one chunk of sequences; returns this thread's inclusive sum, `sum` the chunk's
   auto scan = [&](long long x, long long& sum) {
@@ -220,11 +221,15 @@ __device__ __forceinline__ int slot_of(const Unit& u, int c) {
 constexpr float kSeenInf = -1.0f;
 
 // ---------------------------------------------------------------- host side
-constexpr int kSplitCtas = 2 * kNumSMs;  // most CTAs that a kernel here is launched with
 struct Workspace {
   size_t acc, ml, desc, total;  // offsets and size in bytes
 };
-Workspace workspace(int rows, int head_dim);
+Workspace workspace(int ctas, int rows, int head_dim);
+
+// tcgen05 variant (paged_tree_tc.cu): whether it takes the call, and its launch.
+constexpr int kTcRows = 128;
+bool tc_supported(const Params& p, int q_dtype, int cache_dtype);
+int launch_tc(const Params& p, int q_dtype, int cache_dtype, int ctas, cudaStream_t stream);
 
 }  // namespace tree
 }  // namespace mkv
