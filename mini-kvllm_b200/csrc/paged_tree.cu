@@ -27,7 +27,7 @@ template <typename CT> __device__ __forceinline__ float elem_f32(const uint8_t* 
 }
 
 template <typename QT, typename CT>
-__global__ void __launch_bounds__(kGThreads) paged_tree_generic_kernel(const Params p) {
+__global__ void __launch_bounds__(kGThreads) paged_tree_generic_kernel(const __grid_constant__ Params p) {
   extern __shared__ __align__(16) float sm[];
   const int D = p.head_dim, DK = D + 4;
   float* q_sm = sm;                    // [16][D]
@@ -54,6 +54,7 @@ __global__ void __launch_bounds__(kGThreads) paged_tree_generic_kernel(const Par
     }
     float m[4], l[4], acc[4][8];
     const uint64_t* mrow[4];
+    uint64_t m0[4];
     bool any[4];  // whether the row has seen a token
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
@@ -64,6 +65,7 @@ __global__ void __launch_bounds__(kGThreads) paged_tree_generic_kernel(const Par
       for (int i = 0; i < 8; ++i) acc[r][i] = 0.0f;
       const int R = u.mt * kGRows + min(4 * warp + r, rows - 1);
       mrow[r] = p.mask + (u.s.q0 + R / p.group) * p.mask_st;
+      m0[r] = __ldg(mrow[r]);
     }
     for (int it = u.k0; it < u.k1; ++it) {
       const int t0 = it * kGKT;
@@ -119,7 +121,7 @@ __global__ void __launch_bounds__(kGThreads) paged_tree_generic_kernel(const Par
       float pr[4], alpha[4];
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const uint32_t vis = visible32(u.s, mrow[r], p.mask_words, t0) & page_ok;
+        const uint32_t vis = visible32(u.s, mrow[r], m0[r], p.mask_words, t0) & page_ok;
         any[r] |= vis != 0;
         const bool on = (vis >> lane) & 1;
         const float x = on ? s[r] * sc : -INFINITY;
@@ -195,32 +197,31 @@ constexpr int kCWarps = 4;
 template <typename QT>
 __global__ void __launch_bounds__(32 * kCWarps) paged_tree_combine_kernel(const Params p, int RT) {
   pdl_wait();
-  const int4 d = p.desc[blockIdx.x];
-  if (d.w == 0) return;
-  const Seq s = load_seq(p, d.x);
+  const int4 d = p.desc[2 * blockIdx.x], e = p.desc[2 * blockIdx.x + 1];
+  const int parts_all = d.x, kvh = d.y;
   const int lane = threadIdx.x & 31, row = blockIdx.y * kCWarps + (threadIdx.x >> 5);
-  const int R = d.z * RT + row;
-  if (row >= RT || R >= s.nodes * p.group) return;
+  const int R = d.z + row;
+  if (parts_all == 0 || row >= RT || R >= d.w) return;
   const int c = blockIdx.x, D = p.head_dim;
   auto slot = [&](int i) -> int64_t { return i == 0 ? 2 * (c - 1) + 1 : 2 * (c - 1 + i); };
   float M = -INFINITY;
-  for (int i = lane; i < d.w; i += 32) M = fmaxf(M, p.part_ml[slot(i) * RT + row].x);
+  for (int i = lane; i < parts_all; i += 32) M = fmaxf(M, p.part_ml[slot(i) * RT + row].x);
   M = warp_max(M);
   const float base = M == -INFINITY ? 0.0f : M;
   float L = 0.0f, acc[8];
   bool seen = false;
 #pragma unroll
   for (int i = 0; i < 8; ++i) acc[i] = 0.0f;
-  for (int i0 = 0; i0 < d.w; i0 += 32) {
+  for (int i0 = 0; i0 < parts_all; i0 += 32) {
     float wt = 0.0f, wl = 0.0f;
-    if (i0 + lane < d.w) {  // a part without a visible token has m = -inf and l = 0
+    if (i0 + lane < parts_all) {  // a part without a visible token has m = -inf and l = 0
       const float2 ml = p.part_ml[slot(i0 + lane) * RT + row];
       wt = exp2f(ml.x - base);
       wl = ml.y == kSeenInf ? 0.0f : wt * ml.y;
       seen |= ml.y == kSeenInf;
     }
     L += warp_sum(wl);
-    const int parts = min(32, d.w - i0);
+    const int parts = min(32, parts_all - i0);
 #pragma unroll 4
     for (int i = 0; i < parts; ++i) {
       const float wi = __shfl_sync(0xffffffffu, wt, i);
@@ -232,8 +233,9 @@ __global__ void __launch_bounds__(32 * kCWarps) paged_tree_combine_kernel(const 
   }
   if (__any_sync(0xffffffffu, seen) && M == -INFINITY) L = NAN;
   const int node = R / p.group;
-  QT* o = reinterpret_cast<QT*>(p.out) + (s.q0 + node) * p.o_st +
-          (int64_t)(d.y * p.group + R - node * p.group) * p.o_sh;
+  const int64_t q0 = ((int64_t)e.x << 32) | (uint32_t)e.y;
+  QT* o = reinterpret_cast<QT*>(p.out) + (q0 + node) * p.o_st +
+          (int64_t)(kvh * p.group + R - node * p.group) * p.o_sh;
   const float inv = L == 0.0f ? 0.0f : 1.0f / L;
 #pragma unroll
   for (int j = 0; j < 8; ++j)
@@ -289,7 +291,7 @@ Workspace workspace(int ctas, int rows, int head_dim) {
   w.acc = 0;
   w.ml = up((size_t)2 * ctas * rows * head_dim * 4);
   w.desc = w.ml + up((size_t)2 * ctas * rows * 8);
-  w.total = w.desc + up((size_t)ctas * 16);
+  w.total = w.desc + up((size_t)ctas * 32);
   return w;
 }
 

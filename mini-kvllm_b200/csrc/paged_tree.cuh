@@ -35,7 +35,7 @@ struct Params {
   // split units: partial sums (2 slots per CTA) and one descriptor per CTA
   float* part_acc;  // [slot][row][head_dim], relative to the row's partial maximum
   float2* part_ml;  // [slot][row] = (maximum in the exp2 domain, sum)
-  int4* desc;
+  int4* desc;       // [cta][2]
 };
 
 __device__ __forceinline__ int64_t ld_idx(const void* p, int i64, int64_t i) {
@@ -49,7 +49,7 @@ struct Seq {
   int64_t q0;
   int nodes, len, prefix;
 };
-__device__ __forceinline__ Seq load_seq(const Params& p, int b) {
+static __device__ __noinline__ Seq load_seq(const Params& p, int b) {
   Seq s;
   int64_t a = ld_idx(p.cu, p.cu_i64, b), e = ld_idx(p.cu, p.cu_i64, b + 1);
   a = min(max(a, (int64_t)0), p.total_q);
@@ -69,9 +69,38 @@ __device__ __forceinline__ int64_t load_page(const Params& p, int b, int blk) {
   return (page >= 0 && page < p.num_blocks) ? page : -1;
 }
 
+// The same in two steps: the entry as it lies in memory, loaded well before it is used (with
+// nothing that waits for it), and the page that it means.
+struct Entry {
+  uint32_t lo, hi;
+};
+__device__ __forceinline__ Entry load_entry(const Params& p, int b, int blk) {
+  const int64_t i = (int64_t)b * p.bt_sb + blk;
+  Entry e;
+  if (p.bt_i64) {
+    const uint2 v = __ldg(reinterpret_cast<const uint2*>(p.bt) + i);
+    e.lo = v.x;
+    e.hi = v.y;
+  } else {
+    e.lo = __ldg(reinterpret_cast<const uint32_t*>(p.bt) + i);
+    e.hi = 0;
+  }
+  return e;
+}
+__device__ __forceinline__ void prefetch_entry(const Params& p, int b, int blk) {
+  const char* at = reinterpret_cast<const char*>(p.bt) + (((int64_t)b * p.bt_sb + blk) << (p.bt_i64 ? 3 : 2));
+  asm volatile("prefetch.global.L2 [%0];" ::"l"(at));
+}
+__device__ __forceinline__ int64_t page_of(const Params& p, Entry e) {
+  const int64_t page = p.bt_i64 ? (int64_t)(((uint64_t)e.hi << 32) | e.lo) : (int64_t)(int32_t)e.lo;
+  return (page >= 0 && page < p.num_blocks) ? page : -1;
+}
+
 // Visibility of the 32 tokens t0 .. t0 + 31 for one query row (bit i: token t0 + i): all of
 // the prefix, the tree's nodes by the row's mask, nothing from len on.
-__device__ __forceinline__ uint32_t visible32(const Seq& s, const uint64_t* mask_row, int mask_words, int t0) {
+// mask0: the row's first word, in hand.
+__device__ __forceinline__ uint32_t visible32(const Seq& s, const uint64_t* mask_row, uint64_t mask0, int mask_words,
+                                              int t0) {
   const int in = s.len - t0;  // tokens that exist
   if (in <= 0) return 0u;
   uint32_t v = in >= 32 ? 0xffffffffu : (1u << in) - 1u;
@@ -79,7 +108,8 @@ __device__ __forceinline__ uint32_t visible32(const Seq& s, const uint64_t* mask
   if (j0 <= -32) return v;
   const int first = j0 < 0 ? 0 : j0;
   uint64_t bits = 0;
-  if ((first >> 6) < mask_words) bits = __ldg(mask_row + (first >> 6)) >> (first & 63);
+  if (first < 64) bits = mask0 >> first;
+  else if ((first >> 6) < mask_words) bits = __ldg(mask_row + (first >> 6)) >> (first & 63);
   if ((first & 63) > 32 && (first >> 6) + 1 < mask_words)
     bits |= __ldg(mask_row + (first >> 6) + 1) << (64 - (first & 63));
   uint32_t t = (uint32_t)bits;
@@ -94,12 +124,19 @@ __device__ __forceinline__ uint32_t visible32(const Seq& s, const uint64_t* mask
 // unit that ends inside a CTA's share is written there whole; the parts of a unit that
 // crosses shares go to partial slots (2 c + 1: the part that starts a unit, 2 c: any later
 // one) and are joined by the combine kernel, which takes its orders from desc[c]: the
-// first CTA that continues a unit names the unit's row tile and the number of its parts.
+// first CTA that continues a unit gives the number of its parts, its kv head and first row,
+// and the rows and the first query row of its sequence.
 struct Unit {
   int b, kvh, mt;     // sequence, kv head, row tile
   int k0, k1, tiles;  // token tiles taken here, and of the whole unit
   Seq s;
 };
+
+// a / b of non-negative numbers, in 32 bits where both fit (64-bit division is a long call).
+static __device__ __noinline__ int64_t quot(int64_t a, int64_t b) {
+  if (((uint64_t)a | (uint64_t)b) >> 32 == 0) return (uint32_t)a / (uint32_t)b;
+  return a / b;
+}
 
 template <int RT, int KT>
 __device__ __forceinline__ int64_t items_of(const Params& p, const Seq& s, int& mt, int& kt) {
@@ -109,10 +146,9 @@ __device__ __forceinline__ int64_t items_of(const Params& p, const Seq& s, int& 
 }
 
 struct Walk {
-  int64_t at, end;  // items of this CTA not yet taken
-  int b;
-  int64_t off;      // `at` within sequence b
-  int mt, kt;       // of sequence b
+  int64_t left;    // items of this CTA not yet taken
+  int b, kvh, mt, k;  // the next one
+  int mts, kts;    // row and token tiles of sequence b
   Seq s;
 };
 
@@ -135,7 +171,7 @@ __device__ bool begin(const Params& p, int c, int n, long long* red, Walk& w) {
     if (lane == 31) red[warp] = x;
     __syncthreads();
     sum = 0;
-#pragma unroll
+#pragma unroll 1
     for (int i = 0; i < NT / 32; ++i) {
       if (i < warp) x += red[i];
       sum += red[i];
@@ -148,16 +184,18 @@ __device__ bool begin(const Params& p, int c, int n, long long* red, Walk& w) {
     return items_of<RT, KT>(p, load_seq(p, b), mt, kt);
   };
   long long total = 0, mine = 0, incl = 0, sum;
+#pragma unroll 1
   for (int base = 0; base < p.num_seqs; base += NT) {
     mine = items(base + tid);
     incl = scan(mine, sum);
     total += sum;
   }
   if (n > total) n = (int)total;  // every CTA that works has an item
-  if (tid == 0) p.desc[c] = make_int4(0, 0, 0, 0);
+  if (tid == 0) p.desc[2 * c] = make_int4(0, 0, 0, 0);
   if (c >= n) return false;
-  const int64_t s0 = (int64_t)c * total / n, s1 = (int64_t)(c + 1) * total / n;
+  const int64_t s0 = quot((int64_t)c * total, n), s1 = quot((int64_t)(c + 1) * total, n);
   long long before = 0;
+#pragma unroll 1
   for (int base = 0; base < p.num_seqs; base += NT) {
     if (p.num_seqs > NT) {  // otherwise the first scan still holds
       mine = items(base + tid);
@@ -172,18 +210,21 @@ __device__ bool begin(const Params& p, int c, int n, long long* red, Walk& w) {
     if (before > s0) break;
   }
   __syncthreads();
-  w.at = s0;
-  w.end = s1;
+  w.left = s1 - s0;
   w.b = (int)found[0];
-  w.off = found[1];
+  const int64_t off = found[1];
   w.s = load_seq(p, w.b);
-  items_of<RT, KT>(p, w.s, w.mt, w.kt);
-  const int64_t unit0 = s0 - w.off % w.kt;  // first item of the unit that s0 lies in
-  if (tid == 0 && unit0 < s0 && (int64_t)(c - 1) * total / n <= unit0) {
+  items_of<RT, KT>(p, w.s, w.mts, w.kts);
+  const int64_t i = quot(off, w.kts);
+  w.k = (int)(off - i * w.kts);
+  w.kvh = (int)quot(i, w.mts);
+  w.mt = (int)(i - (int64_t)w.kvh * w.mts);
+  const int64_t unit0 = s0 - w.k;  // first item of the unit that s0 lies in
+  if (tid == 0 && w.k > 0 && quot((int64_t)(c - 1) * total, n) <= unit0) {
     // this CTA is the first to continue the unit: parts from CTA c - 1 to the one holding its last item
-    const int64_t last = ((unit0 + w.kt) * n + total - 1) / total - 1;
-    const int u = (int)(w.off / w.kt);
-    p.desc[c] = make_int4(w.b, u / w.mt, u % w.mt, (int)(last - c + 2));
+    const int64_t last = quot((unit0 + w.kts) * n + total - 1, total) - 1;
+    p.desc[2 * c + 1] = make_int4((int)(w.s.q0 >> 32), (int)w.s.q0, 0, 0);
+    p.desc[2 * c] = make_int4((int)(last - c + 2), w.kvh, w.mt * RT, w.s.nodes * p.group);
   }
   return true;
 }
@@ -191,22 +232,30 @@ __device__ bool begin(const Params& p, int c, int n, long long* red, Walk& w) {
 // The next unit, or the part of it that falls into this CTA's share.
 template <int RT, int KT>
 __device__ __forceinline__ bool next(const Params& p, Walk& w, Unit& u) {
-  if (w.at >= w.end) return false;
-  while (w.off >= (int64_t)p.num_kv_heads * w.mt * w.kt) {  // on to the next sequence that has work
-    w.off -= (int64_t)p.num_kv_heads * w.mt * w.kt;
-    w.s = load_seq(p, ++w.b);
-    items_of<RT, KT>(p, w.s, w.mt, w.kt);
+  if (w.left <= 0) return false;
+  if (w.k == w.kts) {  // on to the next unit
+    w.k = 0;
+    if (++w.mt == w.mts) {
+      w.mt = 0;
+      if (++w.kvh == p.num_kv_heads) {
+        w.kvh = 0;
+#pragma unroll 1
+        do {  // sequences without nodes have no units
+          w.s = load_seq(p, ++w.b);
+          items_of<RT, KT>(p, w.s, w.mts, w.kts);
+        } while (w.mts == 0);
+      }
+    }
   }
-  const int64_t i = w.off / w.kt;
   u.b = w.b;
   u.s = w.s;
-  u.kvh = (int)(i / w.mt);
-  u.mt = (int)(i % w.mt);
-  u.k0 = (int)(w.off % w.kt);
-  u.tiles = w.kt;
-  u.k1 = (int)min((int64_t)w.kt, u.k0 + (w.end - w.at));
-  w.at += u.k1 - u.k0;
-  w.off += u.k1 - u.k0;
+  u.kvh = w.kvh;
+  u.mt = w.mt;
+  u.k0 = w.k;
+  u.tiles = w.kts;
+  u.k1 = (int)min((int64_t)w.kts, w.k + w.left);
+  w.left -= u.k1 - u.k0;
+  w.k = u.k1;
   return true;
 }
 

@@ -9,9 +9,10 @@
 // unit. TMEM: S0 | S1 | O0 | O1, 128 columns each, P (16 bits) over the first half of S.
 //   warp 0      producer: K and V tiles by TMA (one box per page, 128-byte swizzle) into rings
 //   warp 1      MMA issuer: S = Q K^T, O += P V (P from TMEM, V as it lies in its pages)
-//   warps 4-11  softmax of stream 0 (4-7) and 1 (8-11); they stage Q and write the output
+//   warps 2-3   stage the rows of Q, a unit ahead of the products (two buffers)
+//   warps 4-11  softmax of stream 0 (4-7) and 1 (8-11); at a unit's end they join the streams
+//               and write the output, while the products of the next unit start
 //   warps 12-15 8-bit caches: converters of the raw tiles to f16 (exact) for the MMAs
-// (warps 2 and 3 fill the first warpgroup, which gives registers to the softmax ones).
 // K/V bytes are read once per unit of 128 rows; with fewer rows the tensor core's work is
 // padded, which costs nothing while the tile's bytes take longer to arrive (bf16: 64 KB a
 // tile, 1.5 us of an SM's share of HBM; its two products 0.55 us).
@@ -46,25 +47,30 @@ constexpr int kSickSlots = 4;
 template <bool kByte, bool kTok>
 struct Layout {
   static constexpr int kThreads = kByte ? 512 : 384;
-  // registers per thread after the split, of the launch's 512 x 128 or 384 x 168
-  static constexpr int kRegsSoftmax = kByte ? 168 : 200, kRegsOther = kByte ? 88 : 104;
-  static_assert(kByte ? 2 * kRegsSoftmax + 2 * kRegsOther <= 4 * 128 : 2 * kRegsSoftmax + kRegsOther <= 3 * 168,
-                "more registers than the launch has");
-  static constexpr int kKS = kByte ? 2 : 3;  // 16-bit K and V tiles
+  // 16-bit K and V tiles. 8-bit: one K tile is enough, as the next one is converted while the
+  // tensor core works on the values of the tile before
+  static constexpr int kKS = kByte ? 1 : 3;
   static constexpr int kVS = 2;
   static constexpr int kRS = kByte ? 2 : 0;  // raw 8-bit tiles (K and V)
-  static constexpr int Q0 = 0;
-  static constexpr int K0 = Q0 + TILE;
+  static constexpr int Q0 = 0;               // [2]; a free one carries the streams' joint statistics
+  static constexpr int K0 = Q0 + 2 * TILE;
   static constexpr int V0 = K0 + kKS * TILE;
   static constexpr int R0 = V0 + kVS * TILE;
   static constexpr int SC0 = R0 + kRS * 2 * BLK;             // [V stage][K scale, V factor][128]
-  static constexpr int BAR0 = SC0 + (kTok ? kVS * 2 * kTile * 4 : 0);
-  static constexpr int NBAR = 2 * kKS + 2 * kVS + 2 * kRS + 1 + 2 + 2 + 1 + 2 + 1;
-  static constexpr int MISC0 = BAR0 + NBAR * 8;              // tmem base, abort, sick[4], exponents[2]
-  static constexpr int BYTES = MISC0 + 64;
+  static constexpr int QE0 = SC0 + (kTok ? kVS * 2 * kTile * 4 : 0);  // [2][128] exponents of Q's rows
+  static constexpr int BAR0 = QE0 + (kByte ? 2 * kRows : 0);
+  static constexpr int NBAR = 2 * kKS + 2 * kVS + 2 * kRS + 4 + 2 + 2 + 1 + 2 + 1;
+  static constexpr int MISC0 = BAR0 + NBAR * 8;              // tmem base, abort, sick[4], exponents[2], maxima[2][4]
+  static constexpr int BYTES = MISC0 + 80;
   static_assert(BYTES <= 232448, "shared memory per CTA");
   static_assert(kBeginWords(kThreads) * 8 <= TILE, "the schedule's scratch lies in the first K stage");
 };
+
+// A wait that has not been met at once; out of line, as the roles' code should stay small
+// (instructions that one role fetches push out another's).
+__device__ __noinline__ bool wait_on(uint64_t* bar, uint32_t parity, const volatile int* abort) {
+  return mbar_wait(bar, parity, abort);
+}
 
 // 16 bytes of an 8-bit row -> 16 f16 values, exact.
 template <typename CT>
@@ -96,20 +102,13 @@ __device__ __forceinline__ bool clear_sick(uint32_t& w, uint32_t exp) {
   return sick;
 }
 
-template <int N> __device__ __forceinline__ void regs_take() {
-  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
-}
-template <int N> __device__ __forceinline__ void regs_give() {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
-}
-
 __device__ __forceinline__ float pow2f(int e) {  // 2^e, -126 <= e <= 127
   return __uint_as_float((uint32_t)(e + 127) << 23);
 }
 
 template <typename QT, typename CT, bool kTok>
 __global__ void __launch_bounds__((Layout<sizeof(CT) == 1, kTok>::kThreads), 1)
-paged_tree_tc_kernel(const Params p, const __grid_constant__ CUtensorMap kmap,
+paged_tree_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ CUtensorMap kmap,
                      const __grid_constant__ CUtensorMap vmap) {
   constexpr bool kByte = sizeof(CT) == 1;
   using L = Layout<kByte, kTok>;
@@ -117,6 +116,7 @@ paged_tree_tc_kernel(const Params p, const __grid_constant__ CUtensorMap kmap,
   // f16 weights: 2^6 above the reference, so that they stay normal down to 2^-20 of the
   // largest; with the lazy reference (2^8) and a scale factor below 2 they end below 2^15.
   constexpr float kBias = std::is_same<MT, f16>::value ? 6.0f : 0.0f;
+  constexpr bool kToF16 = kByte && std::is_same<QT, bf16>::value;  // Q changes its type
   constexpr int kKS = L::kKS, kVS = L::kVS, kRS = kByte ? L::kRS : 1;
   extern __shared__ __align__(1024) uint8_t smem[];
   uint64_t* kfull = reinterpret_cast<uint64_t*>(smem + L::BAR0);
@@ -126,7 +126,8 @@ paged_tree_tc_kernel(const Params p, const __grid_constant__ CUtensorMap kmap,
   uint64_t* rfull = vempty + kVS;
   uint64_t* rempty = rfull + L::kRS;
   uint64_t* qfull = rempty + L::kRS;
-  uint64_t* sfull = qfull + 1;
+  uint64_t* qempty = qfull + 2;
+  uint64_t* sfull = qempty + 2;
   uint64_t* pfull = sfull + 2;
   uint64_t* ofull = pfull + 2;
   uint64_t* xbar = ofull + 1;
@@ -135,12 +136,11 @@ paged_tree_tc_kernel(const Params p, const __grid_constant__ CUtensorMap kmap,
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::MISC0 + 4);
   volatile int* sick_s = reinterpret_cast<volatile int*>(smem + L::MISC0 + 8);
   volatile int* vexp_s = reinterpret_cast<volatile int*>(smem + L::MISC0 + 8 + 4 * kSickSlots);
+  volatile float* vmax_s = reinterpret_cast<volatile float*>(smem + L::MISC0 + 16 + 4 * kSickSlots);
+  int8_t* qexp_s = reinterpret_cast<int8_t*>(smem + L::QE0);
   float* scales_s = reinterpret_cast<float*>(smem + L::SC0);
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  Walk walk;
-  if (!begin<kRows, kTile, L::kThreads>(p, blockIdx.x, gridDim.x, reinterpret_cast<long long*>(smem + L::K0), walk))
-    return;
   if (tid == 0) {
     for (int s = 0; s < kKS; ++s) {
       mbar_init(&kfull[s], kByte ? 4 : 1);
@@ -154,8 +154,9 @@ paged_tree_tc_kernel(const Params p, const __grid_constant__ CUtensorMap kmap,
       mbar_init(&rfull[s], 1);
       mbar_init(&rempty[s], 4);
     }
-    mbar_init(qfull, 8);
     for (int b = 0; b < 2; ++b) {
+      mbar_init(&qfull[b], 2);
+      mbar_init(&qempty[b], 8);
       mbar_init(&sfull[b], 1);
       mbar_init(&pfull[b], 4);
       mbar_init(&xbar[b], 8);
@@ -167,23 +168,34 @@ paged_tree_tc_kernel(const Params p, const __grid_constant__ CUtensorMap kmap,
     fence_barrier_init();
   }
   if (warp == 1) tmem_alloc(tmem_base_s, kTmemCols);
+  Walk walk;
+  const bool work =
+      begin<kRows, kTile, L::kThreads>(p, blockIdx.x, gridDim.x, reinterpret_cast<long long*>(smem + L::K0), walk);
   tc_fence_before_sync();
   __syncthreads();
   tc_fence_after_sync();
   const uint32_t tmem = *tmem_base_s;
+  if (!work) {
+    if (warp == 1) tmem_dealloc(tmem, kTmemCols);
+    return;
+  }
   // a tile is loaded in segments of one page (or of kTile tokens of a larger page)
   const int seg_rows = p.block_size < kTile ? p.block_size : kTile;
   const int nseg = kTile / seg_rows;
   auto wait = [&](uint64_t* bar, uint32_t phase) -> bool {  // warp-uniform
-    return __all_sync(0xffffffffu, mbar_wait(bar, phase & 1, abort_flag));
+    bool done = mbar_try_wait(bar, phase & 1);
+    if (!done) done = wait_on(bar, phase & 1, abort_flag);
+    return __all_sync(0xffffffffu, done);
   };
-  // page of segment `lane` of tile t, -1 where it is missing or past the context
-  auto seg_page_of = [&](const Unit& u, int t) -> int64_t {
-    const int ts = t * kTile + lane * seg_rows;
-    return (lane < nseg && ts < u.s.len) ? load_page(p, u.b, ts / p.block_size) : -1;
+  const int bs_log2 = 31 - __clz(p.block_size);
+  // table entry of segment `lane` of tile t, and its page: -1 where it is missing or past the context
+  auto seg_in = [&](const Unit& u, int t) -> bool { return lane < nseg && t * kTile + lane * seg_rows < u.s.len; };
+  auto seg_entry = [&](const Unit& u, int t) -> Entry {
+    Entry e{0xffffffffu, 0xffffffffu};
+    if (seg_in(u, t)) e = load_entry(p, u.b, (t * kTile + lane * seg_rows) >> bs_log2);
+    return e;
   };
-  if (warp >= 4 && warp < 12) regs_take<L::kRegsSoftmax>();
-  else regs_give<L::kRegsOther>();
+  auto seg_page = [&](const Unit& u, int t, Entry e) -> int64_t { return seg_in(u, t) ? page_of(p, e) : -1; };
   Unit u;
   uint32_t g = 0;     // tiles of this CTA before the unit's
   uint32_t unit = 0;  // units before this one
@@ -198,6 +210,7 @@ paged_tree_tc_kernel(const Params p, const __grid_constant__ CUtensorMap kmap,
     uint32_t nk = 0, nv = 0;  // K and V tiles issued (8-bit: nk counts both)
     // loads the rows of tile t that exist; the rest of the stage keeps what it held
     auto load = [&](const CUtensorMap* map, int t, int64_t page, uint32_t dst, uint64_t* bar) {
+#pragma unroll 1
       for (int sgi = 0; sgi < nseg; ++sgi) {
         const int64_t pg = __shfl_sync(0xffffffffu, page, sgi);
         if (lane == 0 && pg >= 0) {
@@ -215,11 +228,16 @@ paged_tree_tc_kernel(const Params p, const __grid_constant__ CUtensorMap kmap,
     auto seg_bytes = [&](int64_t page) -> uint32_t {  // of one 8-bit tile or one half of a 16-bit one
       return (uint32_t)__popc(__ballot_sync(0xffffffffu, page >= 0)) * seg_rows * 128u;
     };
+#pragma unroll 1
     while (ok && next<kRows, kTile>(p, walk, u)) {
       const int tiles = u.k1 - u.k0;
       int64_t page_v = -1;
+      Entry next_e = seg_entry(u, u.k0);  // looked up one tile ahead
+#pragma unroll 1
       for (int i = 0; i <= tiles && ok; ++i) {
-        const int64_t page_k = i < tiles ? seg_page_of(u, u.k0 + i) : -1;
+        const int64_t page_k = i < tiles ? seg_page(u, u.k0 + i, next_e) : -1;
+        if (i + 1 < tiles) next_e = seg_entry(u, u.k0 + i + 1);
+        if (i + 8 < tiles && seg_in(u, u.k0 + i + 8)) prefetch_entry(p, u.b, ((u.k0 + i + 8) * kTile + lane * seg_rows) >> bs_log2);
         if constexpr (kByte) {
           if (i == tiles) break;
           const uint32_t st = nk % kRS;
@@ -276,12 +294,12 @@ paged_tree_tc_kernel(const Params p, const __grid_constant__ CUtensorMap kmap,
       if (!wait(&kfull[st], k / kKS)) return false;
       tc_fence_after_sync();
       if (lane == 0) {
-        const uint32_t qaddr = smem_u32(smem + L::Q0), kaddr = smem_u32(smem + L::K0 + st * TILE);
+        const uint64_t qd = smem_desc(smem_u32(smem + L::Q0 + (unit & 1) * TILE), 16, 1024, kLayoutSw128);
+        const uint64_t kd = smem_desc(smem_u32(smem + L::K0 + st * TILE), 16, 1024, kLayoutSw128);
 #pragma unroll
-        for (int c = 0; c < kD / 16; ++c) {  // 16 head_dim columns per MMA
-          const uint32_t off = (c >> 2) * BLK + (c & 3) * 32;
-          mma_f16(tmem + (i & 1) * kTile, smem_desc(qaddr + off, 16, 1024, kLayoutSw128),
-                  smem_desc(kaddr + off, 16, 1024, kLayoutSw128), kIdQK, c > 0 ? 1u : 0u);
+        for (int c = 0; c < kD / 16; ++c) {  // 16 head_dim columns per MMA (descriptors count 16 bytes)
+          const uint32_t off = ((c >> 2) * BLK + (c & 3) * 32) >> 4;
+          mma_f16(tmem + (i & 1) * kTile, qd + off, kd + off, kIdQK, c > 0 ? 1u : 0u);
         }
         mma_commit(&sfull[i & 1]);
         mma_commit(&kempty[st]);
@@ -295,22 +313,25 @@ paged_tree_tc_kernel(const Params p, const __grid_constant__ CUtensorMap kmap,
       ++ns[i & 1];
       tc_fence_after_sync();
       if (lane == 0) {
-        const uint32_t vaddr = smem_u32(smem + L::V0 + st * TILE);
+        const uint64_t vd = smem_desc(smem_u32(smem + L::V0 + st * TILE), BLK, 1024, kLayoutSw128);
 #pragma unroll
         for (int c = 0; c < kTile / 16; ++c)  // 16 tokens per MMA: 8 columns of P
-          mma_f16_ts(tmem + kOCol + (i & 1) * kD, tmem + (i & 1) * kTile + 8 * c,
-                     smem_desc(vaddr + c * 2048, BLK, 1024, kLayoutSw128), kIdPV, (i > 1 || c > 0) ? 1u : 0u);
+          mma_f16_ts(tmem + kOCol + (i & 1) * kD, tmem + (i & 1) * kTile + 8 * c, vd + c * (2048 >> 4), kIdPV,
+                     (i > 1 || c > 0) ? 1u : 0u);
         mma_commit(&vempty[st]);
       }
       __syncwarp();
       return true;
     };
+#pragma unroll 1
     while (ok && next<kRows, kTile>(p, walk, u)) {
       const int tiles = u.k1 - u.k0;
-      ok = wait(qfull, unit) && qk(0) && (tiles < 2 || qk(1));
-      // QK(i + 2) is issued after PV(i), which reads the P that it overwrites; MMAs run in
-      // the order of issue, so its S being full also says that PV(i) is done
-      for (int i = 0; i < tiles && ok; ++i) ok = pv(i) && (i + 2 >= tiles || qk(i + 2));
+      ok = wait(&qfull[unit & 1], unit >> 1);
+      // QK(0), QK(1), PV(0), QK(2), PV(1), ...: QK(i) is issued after PV(i - 2), which reads the P
+      // that it overwrites; MMAs run in the order of issue, so its S being full also says that
+      // PV(i - 2) is done
+#pragma unroll 1
+      for (int i = 0; i < tiles + 2 && ok; ++i) ok = (i < 2 || pv(i - 2)) && (i >= tiles || qk(i));
       if (ok && lane == 0) mma_commit(ofull);
       __syncwarp();
       g += tiles;
@@ -322,9 +343,66 @@ paged_tree_tc_kernel(const Params p, const __grid_constant__ CUtensorMap kmap,
       mbar_wait(drain, 0, nullptr);
     }
     __syncwarp();
-  } else if (warp >= 4 && warp < 12) {
+  } else if (warp < 4) {
+    // ================================================================ rows of Q
+    // (128-byte swizzle, two halves of 64 columns). A negative score scale
+    // turns them around, so that the softmax has a positive one.
+    bool flip = p.qk_scale_log2 < 0.0f;
+    if (kByte && !kTok) flip = flip != (__ldg(p.k_scale) < 0.0f);
+    const uint32_t sign = flip ? 0x80008000u : 0u;
+#pragma unroll 1
+    while (ok && next<kRows, kTile>(p, walk, u)) {
+      if (!(ok = wait(&qempty[unit & 1], (unit >> 1) + 1))) break;
+      const int rows = u.s.nodes * p.group - u.mt * kRows;
+      // 16 lanes a row, 16 bytes each; every load is in flight at once (behind the tiles' bytes a
+      // load takes microseconds)
+      const int c = lane & 15, r0 = 2 * (warp - 2) + (lane >> 4);
+      uint8_t* dst = smem + L::Q0 + (unit & 1) * TILE + (c >> 3) * BLK;
+#pragma unroll 4
+      for (int r = r0; r < kRows; r += 4) {
+        const int R = u.mt * kRows + min(r, rows - 1), node = R / p.group;
+        const QT* src = reinterpret_cast<const QT*>(p.q) + (u.s.q0 + node) * p.q_st +
+                        (int64_t)(u.kvh * p.group + R - node * p.group) * p.q_sh + c * 8;
+        cp_async_16(smem_u32(dst + r * 128 + (((c & 7) ^ (r & 7)) << 4)), src, r < rows ? 16 : 0);
+      }
+      cp_async_commit();
+      cp_async_wait<0>();
+      if (kToF16 || sign != 0) {
+#pragma unroll 4
+        for (int r = r0; r < kRows; r += 4) {
+          uint4* at = reinterpret_cast<uint4*>(dst + r * 128 + (((c & 7) ^ (r & 7)) << 4));
+          uint4 v = *at;
+          float up = 1.0f;
+          if constexpr (kToF16) {
+            // bf16 rows become f16 times a power of two that puts the largest value at 2^14: exact
+            // down to 2^-28 of it
+            auto top = [](uint32_t w) {
+              return fmaxf(fabsf(__uint_as_float(w << 16)), fabsf(__uint_as_float(w & 0xffff0000u)));
+            };
+            float mx = fmaxf(fmaxf(top(v.x), top(v.y)), fmaxf(top(v.z), top(v.w)));
+#pragma unroll
+            for (int o = 8; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+            int e = 0;
+            if (mx > 0.0f) e = min(max(14 - ((int)(__float_as_uint(mx) >> 23) - 127), -100), 100);
+            up = pow2f(e);
+            if (c == 0) qexp_s[(unit & 1) * kRows + r] = (int8_t)e;
+          }
+          auto put = [&](uint32_t w) -> uint32_t {
+            if constexpr (kToF16) w = pack2<f16>(__uint_as_float(w << 16) * up, __uint_as_float(w & 0xffff0000u) * up);
+            return w ^ sign;
+          };
+          *at = make_uint4(put(v.x), put(v.y), put(v.z), put(v.w));
+        }
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&qfull[unit & 1]);
+      ++unit;
+    }
+    if (!ok) *abort_flag = 1;
+  } else if (warp < 12) {
     // ================================================================ softmax
-    const int stream = (warp - 4) >> 2;       // also the half of the columns staged and written
+    const int stream = (warp - 4) >> 2;       // also the half of the columns that it writes
     const int rt = 32 * (warp & 3) + lane;    // row = TMEM lane
     const uint32_t lane_base = (uint32_t)(32 * (warp & 3)) << 16;
     const uint32_t sa = tmem + lane_base + stream * kTile, oa = tmem + lane_base + kOCol;
@@ -335,11 +413,10 @@ paged_tree_tc_kernel(const Params p, const __grid_constant__ CUtensorMap kmap,
       sc0 *= __ldg(p.k_scale);
       vs0 = __ldg(p.v_scale);
     }
-    // the scale is made positive (a negative one turns Q around) and not 0, so that a masked
-    // -inf stays one
-    const bool flip = sc0 < 0.0f;
+    // positive (the rows of Q take a negative sign) and not 0, so that a masked -inf stays one
     sc0 = fabsf(sc0);
     if (sc0 < 1e-30f) sc0 = 1e-30f;
+#pragma unroll 1
     while (ok && next<kRows, kTile>(p, walk, u)) {
       const int tiles = u.k1 - u.k0;
       const int R = u.mt * kRows + rt, rows_left = u.s.nodes * p.group - u.mt * kRows;
@@ -349,76 +426,40 @@ paged_tree_tc_kernel(const Params p, const __grid_constant__ CUtensorMap kmap,
       const int64_t qrow = u.s.q0 + node;
       const int head = u.kvh * p.group + (live ? R - node * p.group : 0);
       const uint64_t* mask_row = p.mask + qrow * p.mask_st;
+      const uint64_t mask0 = __ldg(mask_row);
       float sc = sc0;
-      // ---- this thread's half of the row of Q (128-byte swizzle)
-      {
-        const QT* src = reinterpret_cast<const QT*>(p.q) + qrow * p.q_st + (int64_t)head * p.q_sh;
-        uint8_t* dst = smem + L::Q0 + stream * BLK + rt * 128;
-        float up = 1.0f;
-        if constexpr (kByte && std::is_same<QT, bf16>::value) {
-          // bf16 rows become f16 times a power of two that puts the largest value at 2^14: exact
-          // down to 2^-28 of it
-          float mx = 0.0f;
-          if (live) {
-#pragma unroll 4
-            for (int c = 0; c < 16; ++c) {
-              const uint4 v = *reinterpret_cast<const uint4*>(src + c * 8);
-              const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                mx = fmax3(mx, fabsf(__uint_as_float(w[e] << 16)), fabsf(__uint_as_float(w[e] & 0xffff0000u)));
-            }
-          }
-          if (mx > 0.0f) {
-            const int e = min(max(14 - ((int)(__float_as_uint(mx) >> 23) - 127), -100), 100);
-            up = pow2f(e);
-            sc *= pow2f(-e);
-          }
-        }
-#pragma unroll
-        for (int c = 0; c < 8; ++c) {
-          uint4 v = make_uint4(0u, 0u, 0u, 0u);
-          if (live) v = *reinterpret_cast<const uint4*>(src + stream * 64 + c * 8);
-          uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            if constexpr (kByte && std::is_same<QT, bf16>::value)
-              w[e] = pack2<f16>(__uint_as_float(w[e] << 16) * up, __uint_as_float(w[e] & 0xffff0000u) * up);
-            if (flip) w[e] ^= 0x80008000u;
-          }
-          *reinterpret_cast<uint4*>(dst + ((c ^ (rt & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
-        }
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(qfull);
+      if constexpr (kToF16) {  // the row's power of two
+        if (!(ok = wait(&qfull[unit & 1], unit >> 1))) break;
+        sc *= pow2f(-(int)qexp_s[(unit & 1) * kRows + rt]);
       }
       float m = -INFINITY, l = 0.0f;  // reference (exp2 domain) and sum of this stream
       int vexp = 0;                   // O holds values times 2^-vexp (kTok)
       bool seen = false;
-      int64_t page_next = seg_page_of(u, u.k0 + stream);
+      Entry next_e = seg_entry(u, u.k0 + stream);
+#pragma unroll 1
       for (int i = stream; i < tiles && ok; i += 2) {
         const int t0 = (u.k0 + i) * kTile;
         const uint32_t st = (g + i) % kVS, vph = (g + i) / kVS;
-        const int64_t page = page_next;
-        if (i + 2 < tiles) page_next = seg_page_of(u, u.k0 + i + 2);
+        const int64_t page = seg_page(u, u.k0 + i, next_e);
+        if (i + 2 < tiles) next_e = seg_entry(u, u.k0 + i + 2);
         // ---- what the row sees: everything but in tiles with tree nodes, an end or a missing page
         const uint32_t have = __ballot_sync(0xffffffffu, page >= 0);
-        const bool special = t0 + kTile > u.s.prefix || have != (nseg == 32 ? 0xffffffffu : (1u << nseg) - 1u);
-        uint32_t mw[4];
-        if (special) {
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            mw[k] = visible32(u.s, mask_row, p.mask_words, t0 + 32 * k);
-            uint32_t pm = 0;  // tokens 32k .. 32k + 31 that have a page
-            for (int b = 0; b < 32; b += min(seg_rows, 32))
-              if ((have >> ((32 * k + b) / seg_rows)) & 1u)
-                pm |= (seg_rows >= 32 ? 0xffffffffu : (1u << seg_rows) - 1u) << b;
-            mw[k] &= pm;
-            seen |= mw[k] != 0u;
+        const uint32_t want = __ballot_sync(0xffffffffu, lane < nseg && t0 + lane * seg_rows < u.s.len);
+        const bool special = t0 + kTile > u.s.prefix || have != want;
+        auto visible = [&](int h) -> uint32_t {  // tokens 32 h .. of the tile that the row sees
+          uint32_t vis = visible32(u.s, mask_row, mask0, p.mask_words, t0 + 32 * h);
+          if (have != want) {
+            if (seg_rows >= 32) {
+              if (!((have >> ((32 * h) / seg_rows)) & 1u)) vis = 0;
+            } else {
+#pragma unroll 1
+              for (int b = 0; b < 32; b += seg_rows)
+                if (!((have >> ((32 * h + b) / seg_rows)) & 1u)) vis &= ~(((1u << seg_rows) - 1u) << b);
+            }
           }
-        } else {
-          seen = true;
-        }
+          return vis;
+        };
+        if (!special) seen = true;
         if (!(ok = wait(&sfull[stream], ns))) break;  // also: PV of the stream's previous tile is done
         tc_fence_after_sync();
         const float* ksp = scales_s + st * 2 * kTile;
@@ -436,12 +477,13 @@ paged_tree_tc_kernel(const Params p, const __grid_constant__ CUtensorMap kmap,
           }
         }
         if (warp_live) {
-          auto load_half = [&](int h, float (&v)[64]) {
-            tmem_ld64(sa + 64 * h, v);
+          // 32 scores: times the tokens' K scales, -inf where the row does not see the token
+          auto scores = [&](int h, float (&v)[32]) {
+            tmem_ld32(sa + 32 * h, v);
             if constexpr (kTok) {
 #pragma unroll
-              for (int e = 0; e < 64; e += 4) {
-                const float4 k4 = *reinterpret_cast<const float4*>(ksp + 64 * h + e);
+              for (int e = 0; e < 32; e += 4) {
+                const float4 k4 = *reinterpret_cast<const float4*>(ksp + 32 * h + e);
                 v[e] *= k4.x;
                 v[e + 1] *= k4.y;
                 v[e + 2] *= k4.z;
@@ -449,83 +491,64 @@ paged_tree_tc_kernel(const Params p, const __grid_constant__ CUtensorMap kmap,
               }
             }
             if (special) {
+              const uint32_t vis = visible(h);
+              seen |= vis != 0u;
 #pragma unroll
-              for (int e = 0; e < 64; ++e)
-                if (!((mw[2 * h + (e >> 5)] >> (e & 31)) & 1u)) v[e] = -INFINITY;
+              for (int e = 0; e < 32; ++e)
+                if (!((vis >> e) & 1u)) v[e] = -INFINITY;
             }
           };
-          // P = 2^(s sc - ref) of half h as 16-bit pairs, their sum, the raw maximum
-          auto p_half = [&](int h, float ref, uint32_t (&w)[32], uint64_t (&acc)[2], float (&mx)[4]) {
-            float v[64];
-            load_half(h, v);
+          // the tile's maximum, then P, 32 columns at a time (S is read twice: that costs less
+          // than the registers to hold it, whose spills miss an L1 that shared memory has
+          // taken; and short loops keep the roles' code in the instruction cache)
+          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll 1
+          for (int h = 0; h < 4; ++h) {
+            float v[32];
+            scores(h, v);
 #pragma unroll
-            for (int e = 0; e < 64; e += 8)
+            for (int e = 0; e < 32; e += 8)
 #pragma unroll
               for (int k = 0; k < 4; ++k) mx[k] = fmax3(mx[k], v[e + k], v[e + 4 + k]);
-            const uint64_t sc2 = f2_pack(sc, sc), nref2 = f2_pack(-ref, -ref);
+          }
+          // the reference moves only when a row's maximum has grown by more than 2^8, or is its first
+          const float mt = fmaxf(fmax3(mx[0], mx[1], mx[2]), mx[3]) * sc;
+          const bool need = mt > m + 8.0f;
+          const float m_new = need ? mt : m;
+          const float a2 = need ? exp2f(m - m_new) : 1.0f;  // 0 when m was -inf
+          const float nref = kBias - (m_new == -INFINITY ? 0.0f : m_new);
+          const uint64_t sc2 = f2_pack(sc, sc), nref2 = f2_pack(nref, nref);
+          uint64_t acc[2] = {f2_pack(0.0f, 0.0f), f2_pack(0.0f, 0.0f)};
+#pragma unroll 1
+          for (int h = 0; h < 4; ++h) {
+            float v[32];
+            uint32_t w[16];
+            scores(h, v);
 #pragma unroll
-            for (int e = 0; e < 32; ++e) {
+            for (int e = 0; e < 16; ++e) {
               float x0, x1;
               f2_unpack(f2_fma(f2_pack(v[2 * e], v[2 * e + 1]), sc2, nref2), x0, x1);
               float p0 = ex2_approx(x0), p1 = ex2_approx(x1);  // 0 where masked
               acc[e & 1] = f2_add(acc[e & 1], f2_pack(p0, p1));
               if constexpr (kTok) {
-                const float2 f = *reinterpret_cast<const float2*>(ksp + kTile + 64 * h + 2 * e);
+                const float2 f = *reinterpret_cast<const float2*>(ksp + kTile + 32 * h + 2 * e);
                 p0 *= f.x;
                 p1 *= f.y;
               }
               w[e] = pack2<MT>(p0, p1);
             }
-          };
-          uint32_t w0[32], w1[32];
-          auto p_tile = [&](float ref, float& sum, float& mxr) {
-            uint64_t acc[2] = {f2_pack(0.0f, 0.0f), f2_pack(0.0f, 0.0f)};
-            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-            p_half(0, ref - kBias, w0, acc, mx);
-            reg_fence32(w0);
-            p_half(1, ref - kBias, w1, acc, mx);
-            mxr = fmaxf(fmax3(mx[0], mx[1], mx[2]), mx[3]);
-            float a, b, c, d;
-            f2_unpack(acc[0], a, b);
-            f2_unpack(acc[1], c, d);
-            sum = (a + b) + (c + d);
-          };
-          float sum, mxr;
-          bool need;
-          // P against the reference as it is, together with the tile's maximum; again if a row's
-          // maximum has grown by more than 2^8, or is its first
-          const bool first = __any_sync(0xffffffffu, m == -INFINITY);
-          if (first) {
-            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll 1
-            for (int h = 0; h < 2; ++h) {
-              float v[64];
-              load_half(h, v);
-#pragma unroll
-              for (int e = 0; e < 64; e += 8)
-#pragma unroll
-                for (int k = 0; k < 4; ++k) mx[k] = fmax3(mx[k], v[e + k], v[e + 4 + k]);
-            }
-            mxr = fmaxf(fmax3(mx[0], mx[1], mx[2]), mx[3]);
-          } else {
-            p_tile(m, sum, mxr);
+            tmem_st16u(sa + 16 * h, w);  // over columns of S that have been read
           }
-          const float mt = mxr * sc;
-          need = mt > m + 8.0f;
-          const float m_new = need ? mt : m;
-          const float a2 = need ? exp2f(m - m_new) : 1.0f;  // 0 when m was -inf
-          if (first || __any_sync(0xffffffffu, need)) {
-            float unused;
-            p_tile(m_new == -INFINITY ? 0.0f : m_new, sum, unused);
-          }
+          float s0, s1, s2, s3;
+          f2_unpack(acc[0], s0, s1);
+          f2_unpack(acc[1], s2, s3);
+          const float sum = (s0 + s1) + (s2 + s3);
           if (i > stream) {  // O holds something
             rescale |= __any_sync(0xffffffffu, need);
             alpha *= a2;
           }
           m = m_new;
           l = fmaf(l, a2, sum);
-          tmem_st32(sa, w0);
-          tmem_st32(sa + 32, w1);
           if (rescale) {
 #pragma unroll 1
             for (int c = 0; c < kD / 16; ++c) {
@@ -545,13 +568,13 @@ paged_tree_tc_kernel(const Params p, const __grid_constant__ CUtensorMap kmap,
           const bool exists = t < u.s.len && ((have >> (rt / seg_rows)) & 1u);
           uint8_t* vrow = smem + L::V0 + st * TILE + rt * 128;
           if (!exists) {
-#pragma unroll
+#pragma unroll 4
             for (int k = 0; k < 16; ++k)
               *reinterpret_cast<uint4*>(vrow + (k >> 3) * BLK + (k & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
           } else if (t >= u.s.prefix) {
             constexpr uint32_t kExp = std::is_same<QT, bf16>::value ? 0x7f80u : 0x7c00u;
             bool sick = false;
-#pragma unroll 4
+#pragma unroll 2
             for (int k = 0; k < 16; ++k) {
               uint4* at = reinterpret_cast<uint4*>(vrow + (k >> 3) * BLK + (k & 7) * 16);
               uint4 v = *at;
@@ -571,19 +594,21 @@ paged_tree_tc_kernel(const Params p, const __grid_constant__ CUtensorMap kmap,
         if (lane == 0) mbar_arrive(&pfull[stream]);
         ++ns;
       }
-      // ---- the unit's end: both streams' references and sums change hands in S (free now)
+      // ---- the unit's end: the streams exchange their references and sums
       if (ok) ok = wait(ofull, unit);
       if (!ok) break;
       tc_fence_after_sync();
-      tmem_st4(sa, m, l, (float)vexp, seen ? 1.0f : 0.0f);
-      tc_fence_before_sync();
+      // the products of this unit are done with its Q: its buffer takes the statistics
+      float4* stats = reinterpret_cast<float4*>(smem + L::Q0 + (unit & 1) * TILE);
+      stats[stream * kRows + rt] = make_float4(m, l, (float)vexp, seen ? 1.0f : 0.0f);
       __syncwarp();
       if (lane == 0) mbar_arrive(&xbar[0]);
       if (!(ok = wait(&xbar[0], unit))) break;
-      tc_fence_after_sync();
+      const float4 xs = stats[(stream ^ 1) * kRows + rt];
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&qempty[unit & 1]);
       if (warp_live) {
-        float x[4];
-        tmem_ld4(tmem + lane_base + (stream ^ 1) * kTile, x);
+        const float x[4] = {xs.x, xs.y, xs.z, xs.w};
         const bool both = tiles > 1;
         const float M = both ? fmaxf(m, x[0]) : (stream == 0 ? m : x[0]);
         const float base = M == -INFINITY ? 0.0f : M;
@@ -601,43 +626,45 @@ paged_tree_tc_kernel(const Params p, const __grid_constant__ CUtensorMap kmap,
         float* part = p.part_acc + ((int64_t)(slot < 0 ? 0 : slot) * kRows + rt) * kD + stream * 64;
         const bool sick = sick_s[unit % kSickSlots] == (int)unit + 1;
 #pragma unroll 1
-        for (int c = 0; c < 4; ++c) {
-          float v[16];
-          tmem_ld16(oa + stream * 64 + 16 * c, v);
+        for (int c = 0; c < 2; ++c) {
+          float v[32];
+          tmem_ld32(oa + stream * 64 + 32 * c, v);
 #pragma unroll
-          for (int e = 0; e < 16; ++e) v[e] *= a0;
+          for (int e = 0; e < 32; ++e) v[e] *= a0;
           if (both) {
-            float y[16];
-            tmem_ld16(oa + kD + stream * 64 + 16 * c, y);
+            float y[32];
+            tmem_ld32(oa + kD + stream * 64 + 32 * c, y);
 #pragma unroll
-            for (int e = 0; e < 16; ++e) v[e] = fmaf(y[e], a1, v[e]);
-          }
-          if (sick && live) {  // infinities and NaN of the nodes that the row sees
-#pragma unroll 1
-            for (int t = max(u.s.prefix, u.k0 * kTile); t < min(u.s.len, u.k1 * kTile); ++t) {
-              const int64_t page = load_page(p, u.b, t / p.block_size);
-              if (page < 0 || !(visible32(u.s, mask_row, p.mask_words, t) & 1u)) continue;
-              const int64_t row = (page * p.block_size + (t & (p.block_size - 1))) * p.num_kv_heads + u.kvh;
-              const CT* vr = reinterpret_cast<const CT*>(p.v_cache) + row * kD + stream * 64 + 16 * c;
-              const float f = kTok ? __ldg(p.v_scales + row) : 1.0f;
-#pragma unroll
-              for (int e = 0; e < 16; ++e) {
-                const float x2 = to_f32(vr[e]) * f;
-                if (!isfinite(x2)) v[e] += x2;
-              }
-            }
+            for (int e = 0; e < 32; ++e) v[e] = fmaf(y[e], a1, v[e]);
           }
           if (!live) continue;
           if (slot < 0) {
-            uint32_t w[8];
 #pragma unroll
-            for (int e = 0; e < 16; e += 2) w[e >> 1] = pack2<QT>(v[e] * inv, v[e + 1] * inv);
-            *reinterpret_cast<uint4*>(dst + 16 * c) = make_uint4(w[0], w[1], w[2], w[3]);
-            *reinterpret_cast<uint4*>(dst + 16 * c + 8) = make_uint4(w[4], w[5], w[6], w[7]);
+            for (int e = 0; e < 32; e += 8)
+              *reinterpret_cast<uint4*>(dst + 32 * c + e) =
+                  make_uint4(pack2<QT>(v[e] * inv, v[e + 1] * inv), pack2<QT>(v[e + 2] * inv, v[e + 3] * inv),
+                             pack2<QT>(v[e + 4] * inv, v[e + 5] * inv), pack2<QT>(v[e + 6] * inv, v[e + 7] * inv));
           } else {
 #pragma unroll
-            for (int e = 0; e < 16; e += 4)
-              *reinterpret_cast<float4*>(part + 16 * c + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+            for (int e = 0; e < 32; e += 4)
+              *reinterpret_cast<float4*>(part + 32 * c + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+          }
+        }
+        if (sick && live) {  // infinities and NaN of the nodes that the row sees, added to what was stored
+#pragma unroll 1
+          for (int t = max(u.s.prefix, u.k0 * kTile); t < min(u.s.len, u.k1 * kTile); ++t) {
+            const int64_t page = load_page(p, u.b, t >> bs_log2);
+            if (page < 0 || !(visible32(u.s, mask_row, mask0, p.mask_words, t) & 1u)) continue;
+            const int64_t row = (page * p.block_size + (t & (p.block_size - 1))) * p.num_kv_heads + u.kvh;
+            const CT* vr = reinterpret_cast<const CT*>(p.v_cache) + row * kD + stream * 64;
+            const float f = kTok ? __ldg(p.v_scales + row) : 1.0f;
+#pragma unroll 1
+            for (int e = 0; e < 64; ++e) {
+              const float x2 = to_f32(vr[e]) * f;
+              if (isfinite(x2)) continue;
+              if (slot < 0) dst[e] = from_f32<QT>(to_f32(dst[e]) + x2);
+              else part[e] += x2;
+            }
           }
         }
         if (slot >= 0 && stream == 0 && live)
@@ -657,23 +684,30 @@ paged_tree_tc_kernel(const Params p, const __grid_constant__ CUtensorMap kmap,
     // Thread r converts row r (token t0 + r) of K and V. Rows that do not exist become zeros.
     const int r = 32 * (warp - 12) + lane;
     int vexp = 0;
-    auto row_of = [&](int t) -> int64_t {  // (page, row, head) index of token t, -1
-      if (t >= u.s.len) return -1;
-      const int64_t page = load_page(p, u.b, t / p.block_size);
+    // table entry of token t, and its (page, row, head) index in the cache (-1: none)
+    auto tok_entry = [&](int t) -> Entry {
+      Entry e{0xffffffffu, 0xffffffffu};
+      if (t < u.s.len) e = load_entry(p, u.b, t >> bs_log2);
+      return e;
+    };
+    auto row_of = [&](int t, Entry e) -> int64_t {
+      const int64_t page = t < u.s.len ? page_of(p, e) : -1;
       return page < 0 ? -1 : (page * p.block_size + (t & (p.block_size - 1))) * p.num_kv_heads + u.kvh;
     };
     auto convert = [&](const uint8_t* src, uint8_t* dst, bool valid, bool node) -> bool {
       bool sick = false;
       uint8_t* drow = dst + r * 128;
+      uint4 raw[8];  // all loads first: a store in between would hold the next one back
+#pragma unroll
+      for (int c = 0; c < 8; ++c) raw[c] = *reinterpret_cast<const uint4*>(src + r * 128 + ((c ^ (r & 7)) << 4));
 #pragma unroll
       for (int c = 0; c < 8; ++c) {
-        uint32_t h[8] = {0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u};
-        if (valid) {
-          to_f16x16<CT>(*reinterpret_cast<const uint4*>(src + r * 128 + ((c ^ (r & 7)) << 4)), h);
-          if (node && std::is_same<CT, fp8>::value) {
+        uint32_t h[8];
+        if (!valid) raw[c] = make_uint4(0u, 0u, 0u, 0u);
+        to_f16x16<CT>(raw[c], h);
+        if (node && std::is_same<CT, fp8>::value) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) sick |= clear_sick(h[e], 0x7c00u);
-          }
+          for (int e = 0; e < 8; ++e) sick |= clear_sick(h[e], 0x7c00u);
         }
         const int cc = (c & 3) * 2;  // columns 16c ..: half c / 4, chunks cc and cc + 1
         *reinterpret_cast<uint4*>(drow + (c >> 2) * BLK + ((cc ^ (r & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
@@ -681,19 +715,31 @@ paged_tree_tc_kernel(const Params p, const __grid_constant__ CUtensorMap kmap,
       }
       return sick;
     };
+#pragma unroll 1
     while (ok && next<kRows, kTile>(p, walk, u)) {
       const int tiles = u.k1 - u.k0;
-      int64_t row_next = row_of(u.k0 * kTile + r);
+      // scales are loaded two tiles ahead, table entries three
+      const int tr = u.k0 * kTile + r;
+      auto scale_of = [&](const float* scales, int64_t row) -> float {
+        return kTok && row >= 0 ? __ldg(scales + row) : 0.0f;
+      };
+      Entry e0 = tok_entry(tr), e1 = tok_entry(tr + kTile), next_e = tok_entry(tr + 2 * kTile);
+      int64_t row1 = row_of(tr, e0), row2 = row_of(tr + kTile, e1);
+      float ks1 = scale_of(p.k_scales, row1), vs1 = scale_of(p.v_scales, row1);
+      float ks2 = scale_of(p.k_scales, row2), vs2 = scale_of(p.v_scales, row2);
+#pragma unroll 1
       for (int i = 0; i < tiles && ok; ++i) {
         const uint32_t k = g + i, rs = k % kRS, st = k % kKS, sv = k % kVS;
-        const int t = (u.k0 + i) * kTile + r;
-        const int64_t row = row_next;
-        float ks = 0.0f, vs = 0.0f;
-        if (kTok && row >= 0) {
-          ks = __ldg(p.k_scales + row);
-          vs = __ldg(p.v_scales + row);
-        }
-        if (i + 1 < tiles) row_next = row_of(t + kTile);
+        const int t = tr + i * kTile;
+        const int64_t row = row1;
+        float ks = ks1, vs = vs1;
+        row1 = row2;
+        ks1 = ks2;
+        vs1 = vs2;
+        row2 = row_of(t + 2 * kTile, next_e);
+        ks2 = scale_of(p.k_scales, row2);
+        vs2 = scale_of(p.v_scales, row2);
+        next_e = tok_entry(t + 3 * kTile);
         const bool node = t >= u.s.prefix;
         if (!(ok = wait(&rfull[rs], k / kRS) && wait(&kempty[st], k / kKS + 1))) break;
         const uint8_t* raw = smem + L::R0 + rs * 2 * BLK;
@@ -710,20 +756,18 @@ paged_tree_tc_kernel(const Params p, const __grid_constant__ CUtensorMap kmap,
             vs = 0.0f;
             sick = true;
           }
-          float* mx = scales_s + sv * 2 * kTile;
-          const float a = isfinite(vs) ? fabsf(vs) : 0.0f;
-          const float wm = warp_max(a);
-          // the four warps' maxima, in the K-scale slots they fill next
-          if (lane == 0) mx[32 * (warp - 12)] = wm;
+          const float wm = warp_max(isfinite(vs) ? fabsf(vs) : 0.0f);
+          volatile float* mx = vmax_s + 4 * (k & 1);  // two sets: the other one may still be read
+          if (lane == 0) mx[warp - 12] = wm;
           asm volatile("bar.sync 1, 128;" ::: "memory");
-          const float tm = fmaxf(fmaxf(mx[0], mx[32]), fmaxf(mx[64], mx[96]));
+          const float tm = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
           if (tm > 0.0f) {
             const int e = min(max((int)(__float_as_uint(tm) >> 23) - 127, -100), 100);
             if (e > vexp || e < vexp - 4) vexp = e;
           }
-          asm volatile("bar.sync 1, 128;" ::: "memory");
-          mx[r] = ks;
-          mx[kTile + r] = vs * pow2f(-vexp);
+          float* out = scales_s + sv * 2 * kTile;
+          out[r] = ks;
+          out[kTile + r] = vs * pow2f(-vexp);
           if (r == 0) vexp_s[sv] = vexp;
         }
         if (sick) sick_s[unit % kSickSlots] = (int)unit + 1;
