@@ -594,6 +594,19 @@ MKV_API int mkv_move_kv_rows(void* k_cache, void* v_cache, int32_t cache_dtype, 
                              int32_t index_type, int32_t num_groups, int32_t moves_per_group,
                              int32_t* invalid_count, void* stream);
 
+/*
+ * The five calls above with their arguments, in the same order, as an array of 64-bit words:
+ * pointers and integers as they are, a float as the bits of a double. For bindings in which
+ * every argument of a foreign call has a cost of its own (ctypes: a quarter of a microsecond
+ * each, more than these kernels' launch in sum).
+ */
+#define MKV_CALL_PAGED_TREE_ATTENTION 0
+#define MKV_CALL_TREE_METADATA 1
+#define MKV_CALL_TREE_ACCEPT 2
+#define MKV_CALL_COPY_KV_PAGES 3
+#define MKV_CALL_MOVE_KV_ROWS 4
+MKV_API int mkv_call_packed(int32_t call, const int64_t* args);
+
 #ifdef __cplusplus
 }
 #endif

@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 import threading
 
 PKG_DIR = os.path.dirname(os.path.abspath(__file__))
@@ -22,6 +23,9 @@ DECODE_OVERLAP_PREVIOUS = 2
 NOALLOC_SCRATCH_BYTES = 16 << 20
 AR_MAX_RANKS, AR_MAX_BLOCKS, IPC_HANDLE_BYTES = 8, 128, 64
 AR_FLAG_BYTES = AR_MAX_BLOCKS * AR_MAX_RANKS * 4
+
+CALL_PAGED_TREE_ATTENTION, CALL_TREE_METADATA, CALL_TREE_ACCEPT = 0, 1, 2
+CALL_COPY_KV_PAGES, CALL_MOVE_KV_ROWS = 3, 4
 
 # Every symbol include/mkv.h declares, with (restype, argtypes).
 _p, _i32, _i64, _f32, _sz = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64, ctypes.c_float, ctypes.c_size_t
@@ -82,6 +86,7 @@ SIGNATURES: dict[str, tuple] = {
         _p, _p, _i32, _i32, _i64, _i64, _i32, _i32, _i32, _p, _p, _i64, _p, _p, _i32, _i64, _p, _p]),
     "mkv_move_kv_rows": (ctypes.c_int, [
         _p, _p, _i32, _i32, _i64, _i64, _i32, _i32, _i32, _p, _p, _i64, _p, _p, _i32, _i32, _i32, _p, _p]),
+    "mkv_call_packed": (ctypes.c_int, [_i32, ctypes.c_char_p]),
     "mkv_ipc_alloc": (ctypes.c_int, [_sz, ctypes.POINTER(_p), _p]),
     "mkv_ipc_free": (ctypes.c_int, [_p]),
     "mkv_ipc_open": (ctypes.c_int, [_p, ctypes.POINTER(_p)]),
@@ -122,6 +127,14 @@ def load() -> ctypes.CDLL:
                 fn.argtypes = args
             _lib = lib
     return _lib
+
+
+# Argument words of mkv_call_packed, in the order of the call's parameters (NULL is 0).
+PACK_TREE_ATTENTION = struct.Struct("=29qd6q").pack
+PACK_TREE_METADATA = struct.Struct("=20q").pack
+PACK_TREE_ACCEPT = struct.Struct("=24q").pack
+PACK_COPY_PAGES = struct.Struct("=18q").pack
+PACK_MOVE_ROWS = struct.Struct("=19q").pack
 
 
 def source_hash() -> str:

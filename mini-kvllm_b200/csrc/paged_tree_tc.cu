@@ -293,7 +293,7 @@ paged_tree_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ C
       const uint32_t k = g + i, st = k % kKS;
       if (!wait(&kfull[st], k / kKS)) return false;
       tc_fence_after_sync();
-      if (lane == 0) {
+      if (elect_one()) {
         const uint64_t qd = smem_desc(smem_u32(smem + L::Q0 + (unit & 1) * TILE), 16, 1024, kLayoutSw128);
         const uint64_t kd = smem_desc(smem_u32(smem + L::K0 + st * TILE), 16, 1024, kLayoutSw128);
 #pragma unroll
@@ -312,7 +312,7 @@ paged_tree_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ C
       if (!wait(&pfull[i & 1], ns[i & 1]) || !wait(&vfull[st], v / kVS)) return false;
       ++ns[i & 1];
       tc_fence_after_sync();
-      if (lane == 0) {
+      if (elect_one()) {
         const uint64_t vd = smem_desc(smem_u32(smem + L::V0 + st * TILE), BLK, 1024, kLayoutSw128);
 #pragma unroll
         for (int c = 0; c < kTile / 16; ++c)  // 16 tokens per MMA: 8 columns of P
@@ -332,13 +332,13 @@ paged_tree_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ C
       // PV(i - 2) is done
 #pragma unroll 1
       for (int i = 0; i < tiles + 2 && ok; ++i) ok = (i < 2 || pv(i - 2)) && (i >= tiles || qk(i));
-      if (ok && lane == 0) mma_commit(ofull);
+      if (ok && elect_one()) mma_commit(ofull);
       __syncwarp();
       g += tiles;
       ++unit;
     }
     if (!ok) *abort_flag = 1;
-    if (lane == 0) {  // every MMA done before TMEM is freed
+    if (elect_one()) {  // every MMA done before TMEM is freed
       mma_commit(drain);
       mbar_wait(drain, 0, nullptr);
     }

@@ -252,6 +252,14 @@ __device__ __forceinline__ void tmem_ld4(uint32_t taddr, float (&v)[4]) {
   for (int i = 0; i < 4; ++i) v[i] = __uint_as_float(r[i]);
 }
 
+// One lane of a converged warp, chosen by the hardware: the branch on it is known to be
+// uniform, so the operands of what it guards can live in uniform registers.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\tselp.u32 %0, 1, 0, e;\n\t}" : "=r"(p));
+  return p != 0;
+}
+
 // ---------------------------------------------------------------- descriptors
 // Shared-memory matrix descriptor: start address, leading / stride byte offsets (in
 // bytes, multiples of 16), version 1, swizzle layout (0 none, 2 = 128-byte swizzle).

@@ -31,7 +31,7 @@ from typing import Iterable, Optional, Sequence
 import torch
 
 from .. import _lib
-from ..layers.attention import _INDEX, _DTYPES, _on_device, _require_cuda, _stream
+from ..layers.attention import _INDEX, _DTYPES, _call_packed, _device_index
 
 PER_TOKEN_HEAD = ("fp8_per_token_head", "int8_per_token_head")
 QUANTIZED = ("fp8_per_tensor",) + PER_TOKEN_HEAD
@@ -266,17 +266,17 @@ def tree_metadata(parents: torch.Tensor, cu_seqlens_q: torch.Tensor, prefix_lens
     fn = "tree_metadata"
     if not 1 <= max_nodes <= 1024:
         raise ValueError(f"{fn}: max_nodes must be 1 to 1024 (got {max_nodes})")
-    dev = _require_cuda(fn, parents, cu_seqlens_q, prefix_lens, block_tables)
+    idx = _device_index(fn, parents, cu_seqlens_q, prefix_lens, block_tables)
     keep, args = _tree_args(fn, parents, cu_seqlens_q, prefix_lens, block_tables, block_size)
     B, total, words = args[-2], args[-1], (max_nodes + 63) // 64
-    slots = torch.empty(total, dtype=torch.int64, device=dev)
-    lens = torch.empty(B, dtype=torch.int64, device=dev)
-    positions = torch.empty(total, dtype=torch.int64, device=dev)
-    mask = torch.empty(total, words, dtype=torch.int64, device=dev)
-    with _on_device(dev):
-        st = _lib.load().mkv_tree_metadata(*args, words, slots.data_ptr(), lens.data_ptr(),
-                                           positions.data_ptr(), mask.data_ptr(), None, _stream(dev))
-    _lib.check(fn, st)
+    slots = parents.new_empty(total, dtype=torch.int64)
+    lens = parents.new_empty(B, dtype=torch.int64)
+    positions = parents.new_empty(total, dtype=torch.int64)
+    mask = parents.new_empty((total, words), dtype=torch.int64)
+    st = _call_packed(_lib.load(), idx, _lib.CALL_TREE_METADATA, _lib.PACK_TREE_METADATA, args + (
+        words, slots.data_ptr(), lens.data_ptr(), positions.data_ptr(), mask.data_ptr(), 0))
+    if st:
+        _lib.check(fn, st)
     return TreeMetadata(slots, lens, positions, mask)
 
 
@@ -290,7 +290,7 @@ def tree_accept(draft_tokens: torch.Tensor, target_tokens: torch.Tensor, parents
     tokens to keep, and the moves that bring the accepted rows there (move_kv_rows). The
     other arguments as for tree_metadata."""
     fn = "tree_accept"
-    dev = _require_cuda(fn, draft_tokens, target_tokens, parents, cu_seqlens_q, prefix_lens, block_tables)
+    idx = _device_index(fn, draft_tokens, target_tokens, parents, cu_seqlens_q, prefix_lens, block_tables)
     draft, target = _indices(fn, "draft_tokens", draft_tokens, 1), _indices(fn, "target_tokens", target_tokens, 1)
     keep, args = _tree_args(fn, parents, cu_seqlens_q, prefix_lens, block_tables, block_size)
     B, total = args[-2], args[-1]
@@ -298,20 +298,17 @@ def tree_accept(draft_tokens: torch.Tensor, target_tokens: torch.Tensor, parents
         raise ValueError(f"{fn}: draft_tokens and target_tokens must be {total} tokens each, of one dtype")
     if max_path < 1:
         raise ValueError(f"{fn}: max_path must be at least 1 (got {max_path})")
-    # (B, max_path) rows of int64, then of int32, and the two counts, in one allocation each
-    wide = torch.empty(B * (3 * max_path + 1), dtype=torch.int64, device=dev)
-    narrow = torch.empty(B * (max_path + 1), dtype=torch.int32, device=dev)
-    n = B * max_path
-    tokens, src, dst, lens = wide[:n], wide[n:2 * n], wide[2 * n:3 * n], wide[3 * n:]
-    nodes, count = narrow[:n], narrow[n:]
-    with _on_device(dev):
-        st = _lib.load().mkv_tree_accept(
-            draft.data_ptr(), target.data_ptr(), _INDEX[draft.dtype], *args, max_path, count.data_ptr(),
-            nodes.data_ptr(), tokens.data_ptr(), lens.data_ptr(), src.data_ptr(), dst.data_ptr(),
-            _stream(dev))
-    _lib.check(fn, st)
-    shape = (B, max_path)
-    return TreeAcceptance(count, nodes.view(shape), tokens.view(shape), lens, src.view(shape), dst.view(shape))
+    tokens, src, dst = parents.new_empty((3, B, max_path), dtype=torch.int64).unbind(0)
+    nodes = parents.new_empty((B, max_path), dtype=torch.int32)
+    count = parents.new_empty(B, dtype=torch.int32)
+    lens = parents.new_empty(B, dtype=torch.int64)
+    st = _call_packed(_lib.load(), idx, _lib.CALL_TREE_ACCEPT, _lib.PACK_TREE_ACCEPT, (
+        draft.data_ptr(), target.data_ptr(), _INDEX[draft.dtype]) + args + (
+        max_path, count.data_ptr(), nodes.data_ptr(), tokens.data_ptr(), lens.data_ptr(), src.data_ptr(),
+        dst.data_ptr()))
+    if st:
+        _lib.check(fn, st)
+    return TreeAcceptance(count, nodes, tokens, lens, src, dst)
 
 
 # ------------------------------------------------------------------ copies inside the cache
@@ -322,8 +319,7 @@ def _cache_args(fn: str, cache: KVCache):
     if kv.dtype not in _DTYPES:
         raise ValueError(f"{fn}: unsupported cache dtype {kv.dtype}")
     _, L, NB, BS, KVH, D = kv.shape
-    ks = vs = None
-    stride = 0
+    ks = vs = stride = 0
     if cache.kv_cache_dtype in PER_TOKEN_HEAD:
         for t in (cache.k_scale, cache.v_scale):
             if t is None or t.dtype != torch.float32 or t.shape != (L, NB, BS, KVH) or not t.is_contiguous():
@@ -335,14 +331,13 @@ def _cache_args(fn: str, cache: KVCache):
 
 
 def _pairs(fn: str, cache: KVCache, src: torch.Tensor, dst: torch.Tensor, dim: int):
-    tensors = (cache.kv, src, dst)
-    if cache.kv_cache_dtype in PER_TOKEN_HEAD and cache.k_scale is not None and cache.v_scale is not None:
-        tensors += (cache.k_scale, cache.v_scale)
-    dev = _require_cuda(fn, *tensors)
+    scales = cache.kv_cache_dtype in PER_TOKEN_HEAD
+    idx = _device_index(fn, cache.kv, src, dst, cache.k_scale if scales else None,
+                        cache.v_scale if scales else None)
     src, dst = _indices(fn, "the source", src, dim), _indices(fn, "the destination", dst, dim)
     if src.shape != dst.shape or src.dtype != dst.dtype:
         raise ValueError(f"{fn}: source and destination must have one shape and dtype")
-    return dev, src, dst
+    return idx, src, dst
 
 
 def copy_kv_pages(cache: KVCache, src_pages: torch.Tensor, dst_pages: torch.Tensor) -> None:
@@ -352,12 +347,11 @@ def copy_kv_pages(cache: KVCache, src_pages: torch.Tensor, dst_pages: torch.Tens
     written by an earlier one sees what was written; an entry below 0 is no copy, one past
     the cache is skipped."""
     fn = "copy_kv_pages"
-    dev, src, dst = _pairs(fn, cache, src_pages, dst_pages, 1)
-    args = _cache_args(fn, cache)
-    with _on_device(dev):
-        st = _lib.load().mkv_copy_kv_pages(*args, src.data_ptr(), dst.data_ptr(), _INDEX[src.dtype],
-                                           src.numel(), None, _stream(dev))
-    _lib.check(fn, st)
+    idx, src, dst = _pairs(fn, cache, src_pages, dst_pages, 1)
+    st = _call_packed(_lib.load(), idx, _lib.CALL_COPY_KV_PAGES, _lib.PACK_COPY_PAGES, _cache_args(fn, cache) + (
+        src.data_ptr(), dst.data_ptr(), _INDEX[src.dtype], src.numel(), 0))
+    if st:
+        _lib.check(fn, st)
 
 
 def move_kv_rows(cache: KVCache, src_slots: torch.Tensor, dst_slots: torch.Tensor) -> None:
@@ -368,12 +362,11 @@ def move_kv_rows(cache: KVCache, src_slots: torch.Tensor, dst_slots: torch.Tenso
     writes no other may read or write. An entry below 0 is no move, one past the cache is
     skipped."""
     fn = "move_kv_rows"
-    dev, src, dst = _pairs(fn, cache, src_slots, dst_slots, 2)
-    args = _cache_args(fn, cache)
-    with _on_device(dev):
-        st = _lib.load().mkv_move_kv_rows(*args, src.data_ptr(), dst.data_ptr(), _INDEX[src.dtype],
-                                          src.shape[0], src.shape[1], None, _stream(dev))
-    _lib.check(fn, st)
+    idx, src, dst = _pairs(fn, cache, src_slots, dst_slots, 2)
+    st = _call_packed(_lib.load(), idx, _lib.CALL_MOVE_KV_ROWS, _lib.PACK_MOVE_ROWS, _cache_args(fn, cache) + (
+        src.data_ptr(), dst.data_ptr(), _INDEX[src.dtype], src.shape[0], src.shape[1], 0))
+    if st:
+        _lib.check(fn, st)
 
 
 def kv_head_shard(num_heads: int, num_kv_heads: int, rank: int, world_size: int):

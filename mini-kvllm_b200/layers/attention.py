@@ -90,6 +90,29 @@ def _stream(device: torch.device) -> ctypes.c_void_p:
     return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
 
 
+def _device_index(fn: str, *tensors: torch.Tensor | None) -> int:
+    """The device that all the tensors are on (None entries left out)."""
+    idx = tensors[0].get_device()
+    for t in tensors:
+        if t is not None and (t.get_device() != idx or idx < 0):
+            _require_cuda(fn, *[x for x in tensors if x is not None])
+    return idx
+
+
+def _call_packed(lib, idx: int, call: int, pack, args: tuple) -> int:
+    """mkv_call_packed of `args` and the current stream of device `idx`, with that device
+    current. (torch._C's raw calls: the public ones build a Stream object and cost several
+    microseconds, as much as the launch.)"""
+    cur = torch._C._cuda_getDevice()
+    if cur == idx:
+        return lib.mkv_call_packed(call, pack(*args, torch._C._cuda_getCurrentRawStream(idx)))
+    torch.cuda.set_device(idx)
+    try:
+        return lib.mkv_call_packed(call, pack(*args, torch._C._cuda_getCurrentRawStream(idx)))
+    finally:
+        torch.cuda.set_device(cur)
+
+
 def _index_tensor(t: torch.Tensor, fn: str, what: str) -> torch.Tensor:
     if t.dtype not in _INDEX:
         raise ValueError(f"{fn}: {what} must be int32 or int64 (got {t.dtype})")
@@ -571,19 +594,17 @@ def paged_attention_tree(query: torch.Tensor, k_cache: torch.Tensor, v_cache: to
         raise ValueError(f"{fn}: query must be (total_q, {num_heads}, {head_dim}), got {tuple(query.shape)}")
     if query.dtype not in _FLOAT_IO:
         raise ValueError(f"{fn}: unsupported query dtype {query.dtype}")
-    tensors = [query, k_cache, v_cache, block_tables, context_lens, cu_seqlens_q, tree_mask]
     quant = kv_cache_dtype != "auto"
     if quant:
         if kv_cache_dtype not in ("fp8_per_tensor",) + _PER_TOKEN_HEAD:
             raise NotImplementedError(f"{fn}: kv_cache_dtype {kv_cache_dtype!r} is not implemented")
         if k_scale is None or v_scale is None:
             raise ValueError(f"{fn}: {kv_cache_dtype} needs k_scale and v_scale")
-        tensors += [k_scale, v_scale]
-    if out is not None:
-        if out.shape != query.shape or out.dtype != query.dtype or (out.numel() and out.stride(-1) != 1):
-            raise ValueError(f"{fn}: out must have the query's shape and dtype, and contiguous rows")
-        tensors.append(out)
-    dev = _require_cuda(fn, *tensors)
+    if out is not None and (out.shape != query.shape or out.dtype != query.dtype or
+                            (out.numel() and out.stride(-1) != 1)):
+        raise ValueError(f"{fn}: out must have the query's shape and dtype, and contiguous rows")
+    idx = _device_index(fn, query, k_cache, v_cache, block_tables, context_lens, cu_seqlens_q, tree_mask,
+                        k_scale if quant else None, v_scale if quant else None, out)
     total_q, num_seqs = query.shape[0], context_lens.numel()
     if tree_mask.dtype != torch.int64 or tree_mask.dim() != 2 or tree_mask.shape[0] != total_q or \
             tree_mask.shape[1] < 1:
@@ -591,12 +612,12 @@ def paged_attention_tree(query: torch.Tensor, k_cache: torch.Tensor, v_cache: to
                          f"{tuple(tree_mask.shape)}")
     if block_tables.dim() != 2 or block_tables.dtype not in _INDEX:
         raise ValueError(f"{fn}: block_tables must be a two-dimensional int32 or int64 tensor")
-    lens = _index_tensor(context_lens.reshape(-1), fn, "context_lens")
-    cu = _index_tensor(cu_seqlens_q.reshape(-1), fn, "cu_seqlens_q")
+    lens = _index_tensor(context_lens if context_lens.dim() == 1 else context_lens.reshape(-1), fn, "context_lens")
+    cu = _index_tensor(cu_seqlens_q if cu_seqlens_q.dim() == 1 else cu_seqlens_q.reshape(-1), fn, "cu_seqlens_q")
     if cu.numel() != num_seqs + 1 or block_tables.shape[0] < num_seqs:
         raise ValueError(f"{fn}: cu_seqlens_q/block_tables do not match {num_seqs} sequences")
     num_blocks = _check_cache(fn, k_cache, v_cache, block_size, num_kv_heads, head_dim)
-    kp = vp = kps = vps = None
+    kp = vp = kps = vps = 0
     if not quant:
         if k_cache.dtype != query.dtype:
             raise ValueError(f"{fn}: cache dtype {k_cache.dtype} must equal the query dtype {query.dtype}")
@@ -610,38 +631,43 @@ def paged_attention_tree(query: torch.Tensor, k_cache: torch.Tensor, v_cache: to
         kp, vp = k_scale.data_ptr(), v_scale.data_ptr()
         cache_code = _lib.DTYPE_FP8_E4M3
     else:
-        want = torch.int8 if kv_cache_dtype.startswith("int8") else torch.float8_e4m3fn
+        want = torch.int8 if kv_cache_dtype == "int8_per_token_head" else torch.float8_e4m3fn
         if k_cache.dtype != want:
             raise ValueError(f"{fn}: {kv_cache_dtype} needs {want} caches (got {k_cache.dtype})")
         _check_row_scales(fn, k_scale, v_scale, num_blocks, block_size, num_kv_heads)
         kps, vps = k_scale.data_ptr(), v_scale.data_ptr()
         cache_code = _DTYPES[want]
-    output = out if out is not None else torch.empty(query.shape, dtype=query.dtype, device=dev)
+    output = out if out is not None else query.new_empty(query.shape)
     if total_q == 0 or num_seqs == 0:
         return output
-    if query.stride(-1) != 1:
+    qs = query.stride()
+    if qs[2] != 1:
         query = query.contiguous()
-    if block_tables.stride(-1) != 1:
+        qs = query.stride()
+    bs = block_tables.stride()
+    if bs[1] != 1:
         block_tables = block_tables.contiguous()
-    if tree_mask.stride(-1) != 1:
+        bs = block_tables.stride()
+    ms = tree_mask.stride()
+    if ms[1] != 1:
         tree_mask = tree_mask.contiguous()
+        ms = tree_mask.stride()
+    os_ = output.stride()
     lib = _lib.load()
     dt = _DTYPES[query.dtype]
     ws_n = lib.mkv_paged_tree_workspace_bytes(num_seqs, total_q, num_heads, num_kv_heads, head_dim, dt,
                                               cache_code)
     # from the caching allocator at each call: calls on other streams, and captured graphs,
     # never share a workspace
-    ws = torch.empty(ws_n, dtype=torch.uint8, device=dev)
-    with _on_device(dev):
-        st = lib.mkv_paged_tree_attention(
-            query.data_ptr(), query.stride(0), query.stride(1), dt, k_cache.data_ptr(),
-            v_cache.data_ptr(), cache_code, kp, vp, kps, vps, num_blocks, block_size,
-            block_tables.data_ptr(), _INDEX[block_tables.dtype], block_tables.stride(0),
-            block_tables.shape[1], lens.data_ptr(), _INDEX[lens.dtype], cu.data_ptr(),
-            _INDEX[cu.dtype], tree_mask.data_ptr(), tree_mask.stride(0), tree_mask.shape[1], num_seqs,
-            total_q, num_heads, num_kv_heads, head_dim, float(scale), output.data_ptr(),
-            output.stride(0), output.stride(1), ws.data_ptr(), ws_n, _stream(dev))
-    _lib.check(fn, st)
+    ws = query.new_empty(ws_n, dtype=torch.uint8)
+    st = _call_packed(lib, idx, _lib.CALL_PAGED_TREE_ATTENTION, _lib.PACK_TREE_ATTENTION, (
+        query.data_ptr(), qs[0], qs[1], dt, k_cache.data_ptr(), v_cache.data_ptr(), cache_code, kp, vp,
+        kps, vps, num_blocks, block_size, block_tables.data_ptr(), _INDEX[block_tables.dtype], bs[0],
+        block_tables.shape[1], lens.data_ptr(), _INDEX[lens.dtype], cu.data_ptr(), _INDEX[cu.dtype],
+        tree_mask.data_ptr(), ms[0], tree_mask.shape[1], num_seqs, total_q, num_heads, num_kv_heads,
+        head_dim, float(scale), output.data_ptr(), os_[0], os_[1], ws.data_ptr(), ws_n))
+    if st:
+        _lib.check(fn, st)
     return output
 
 
