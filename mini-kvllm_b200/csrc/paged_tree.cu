@@ -307,7 +307,7 @@ extern "C" size_t mkv_paged_tree_workspace_bytes(int32_t num_seqs, int64_t total
   // the larger of the two kernels' (which of them runs depends on the tensors' alignment too)
   const size_t generic = tree::workspace(tree::kGCtas, tree::kGRows, head_dim).total;
   const size_t tc = tree::workspace(kNumSMs, tree::kTcRows, head_dim).total;
-  return head_dim == 128 && q_dtype != MKV_DTYPE_F32 && tc > generic ? tc : generic;
+  return (head_dim == 128 || head_dim == 64) && q_dtype != MKV_DTYPE_F32 && tc > generic ? tc : generic;
 }
 
 extern "C" int mkv_paged_tree_attention(

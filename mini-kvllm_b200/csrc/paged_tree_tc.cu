@@ -1,4 +1,4 @@
-// Tree attention on the 5th-generation tensor cores: 16-bit queries, head_dim 128, pages of
+// Tree attention on the 5th-generation tensor cores: 16-bit queries, head_dim 64 or 128, pages of
 // a power of two >= 8 tokens; caches in the query's dtype, e4m3 or int8.
 //
 // A persistent CTA per SM takes an even share of the token tiles (paged_tree.cuh). A unit is
@@ -37,15 +37,16 @@ namespace tree {
 namespace {
 using namespace sm100;
 
-constexpr int kRows = kTcRows, kTile = 128, kD = 128;
-constexpr int BLK = 128 * 128;   // 128 rows x 128 bytes
-constexpr int TILE = 2 * BLK;    // a 16-bit tile: two halves of 64 columns
+constexpr int kRows = kTcRows, kTile = 128;
+constexpr int BLK = 128 * 128;  // 128 rows x 128 bytes: 64 columns of a 16-bit tile
 constexpr uint32_t kTmemCols = 512, kOCol = 256;
 constexpr int kSickSlots = 4;
 
 // kByte: 8-bit cache; kTok: with per-(token, head) scales.
-template <bool kByte, bool kTok>
+template <bool kByte, bool kTok, int kD>
 struct Layout {
+  static constexpr int TILE = kD / 64 * BLK;  // a 16-bit tile
+  static constexpr int RAW = kTile * kD;      // an 8-bit one
   static constexpr int kThreads = kByte ? 512 : 384;
   // 16-bit K and V tiles. 8-bit: one K tile is enough, as the next one is converted while the
   // tensor core works on the values of the tile before
@@ -56,7 +57,7 @@ struct Layout {
   static constexpr int K0 = Q0 + 2 * TILE;
   static constexpr int V0 = K0 + kKS * TILE;
   static constexpr int R0 = V0 + kVS * TILE;
-  static constexpr int SC0 = R0 + kRS * 2 * BLK;             // [V stage][K scale, V factor][128]
+  static constexpr int SC0 = R0 + kRS * 2 * RAW;             // [V stage][K scale, V factor][128]
   static constexpr int QE0 = SC0 + (kTok ? kVS * 2 * kTile * 4 : 0);  // [2][128] exponents of Q's rows
   static constexpr int BAR0 = QE0 + (kByte ? 2 * kRows : 0);
   static constexpr int NBAR = 2 * kKS + 2 * kVS + 2 * kRS + 4 + 2 + 2 + 1 + 2 + 1;
@@ -106,12 +107,13 @@ __device__ __forceinline__ float pow2f(int e) {  // 2^e, -126 <= e <= 127
   return __uint_as_float((uint32_t)(e + 127) << 23);
 }
 
-template <typename QT, typename CT, bool kTok>
-__global__ void __launch_bounds__((Layout<sizeof(CT) == 1, kTok>::kThreads), 1)
+template <typename QT, typename CT, bool kTok, int kD>
+__global__ void __launch_bounds__((Layout<sizeof(CT) == 1, kTok, kD>::kThreads), 1)
 paged_tree_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ CUtensorMap kmap,
                      const __grid_constant__ CUtensorMap vmap) {
   constexpr bool kByte = sizeof(CT) == 1;
-  using L = Layout<kByte, kTok>;
+  using L = Layout<kByte, kTok, kD>;
+  constexpr int TILE = L::TILE;
   using MT = typename std::conditional<kByte, f16, QT>::type;  // operands of the MMAs
   // f16 weights: 2^6 above the reference, so that they stay normal down to 2^-20 of the
   // largest; with the lazy reference (2^8) and a scale factor below 2 they end below 2^15.
@@ -215,18 +217,14 @@ paged_tree_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ C
         const int64_t pg = __shfl_sync(0xffffffffu, page, sgi);
         if (lane == 0 && pg >= 0) {
           const int y = (int)(pg * p.block_size) + ((t * kTile + sgi * seg_rows) & (p.block_size - 1));
-          if constexpr (kByte) {
-            tma_load_2d(dst + sgi * seg_rows * 128, map, u.kvh * kD, y, bar);
-          } else {
-            tma_load_2d(dst + sgi * seg_rows * 128, map, u.kvh * kD, y, bar);
-            tma_load_2d(dst + BLK + sgi * seg_rows * 128, map, u.kvh * kD + 64, y, bar);
-          }
+          tma_load_2d(dst + sgi * seg_rows * (kByte ? kD : 128), map, u.kvh * kD, y, bar);
+          if constexpr (!kByte && kD == 128) tma_load_2d(dst + BLK + sgi * seg_rows * 128, map, u.kvh * kD + 64, y, bar);
         }
       }
       __syncwarp();
     };
-    auto seg_bytes = [&](int64_t page) -> uint32_t {  // of one 8-bit tile or one half of a 16-bit one
-      return (uint32_t)__popc(__ballot_sync(0xffffffffu, page >= 0)) * seg_rows * 128u;
+    auto seg_bytes = [&](int64_t page) -> uint32_t {  // of one tile
+      return (uint32_t)__popc(__ballot_sync(0xffffffffu, page >= 0)) * (uint32_t)(seg_rows * kD * (int)sizeof(CT));
     };
 #pragma unroll 1
     while (ok && next<kRows, kTile>(p, walk, u)) {
@@ -245,15 +243,15 @@ paged_tree_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ C
           const uint32_t bytes = 2 * seg_bytes(page_k);
           if (lane == 0) mbar_arrive_expect_tx(&rfull[st], bytes);
           __syncwarp();
-          const uint32_t dst = smem_u32(smem + L::R0 + st * 2 * BLK);
+          const uint32_t dst = smem_u32(smem + L::R0 + st * 2 * L::RAW);
           load(&kmap, u.k0 + i, page_k, dst, &rfull[st]);
-          load(&vmap, u.k0 + i, page_k, dst + BLK, &rfull[st]);
+          load(&vmap, u.k0 + i, page_k, dst + L::RAW, &rfull[st]);
           ++nk;
         } else {  // K one tile ahead of V, the order in which the products take them
           if (i < tiles) {
             const uint32_t st = nk % kKS;
             if (!(ok = wait(&kempty[st], nk / kKS + 1))) break;
-            const uint32_t bytes = 2 * seg_bytes(page_k);
+            const uint32_t bytes = seg_bytes(page_k);
             if (lane == 0) mbar_arrive_expect_tx(&kfull[st], bytes);
             __syncwarp();
             load(&kmap, u.k0 + i, page_k, smem_u32(smem + L::K0 + st * TILE), &kfull[st]);
@@ -262,7 +260,7 @@ paged_tree_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ C
           if (i > 0) {
             const uint32_t st = nv % kVS;
             if (!(ok = wait(&vempty[st], nv / kVS + 1))) break;
-            const uint32_t bytes = 2 * seg_bytes(page_v);
+            const uint32_t bytes = seg_bytes(page_v);
             if (lane == 0) mbar_arrive_expect_tx(&vfull[st], bytes);
             __syncwarp();
             load(&vmap, u.k0 + i - 1, page_v, smem_u32(smem + L::V0 + st * TILE), &vfull[st]);
@@ -354,12 +352,13 @@ paged_tree_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ C
     while (ok && next<kRows, kTile>(p, walk, u)) {
       if (!(ok = wait(&qempty[unit & 1], (unit >> 1) + 1))) break;
       const int rows = u.s.nodes * p.group - u.mt * kRows;
-      // 16 lanes a row, 16 bytes each; every load is in flight at once (behind the tiles' bytes a
+      // 16 bytes a lane; every load is in flight at once (behind the tiles' bytes a
       // load takes microseconds)
-      const int c = lane & 15, r0 = 2 * (warp - 2) + (lane >> 4);
+      constexpr int kLanes = kD / 8, kStep = 64 / kLanes;  // lanes of a row, rows of a round
+      const int c = lane % kLanes, r0 = (32 / kLanes) * (warp - 2) + lane / kLanes;
       uint8_t* dst = smem + L::Q0 + (unit & 1) * TILE + (c >> 3) * BLK;
 #pragma unroll 4
-      for (int r = r0; r < kRows; r += 4) {
+      for (int r = r0; r < kRows; r += kStep) {
         const int R = u.mt * kRows + min(r, rows - 1), node = R / p.group;
         const QT* src = reinterpret_cast<const QT*>(p.q) + (u.s.q0 + node) * p.q_st +
                         (int64_t)(u.kvh * p.group + R - node * p.group) * p.q_sh + c * 8;
@@ -369,7 +368,7 @@ paged_tree_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ C
       cp_async_wait<0>();
       if (kToF16 || sign != 0) {
 #pragma unroll 4
-        for (int r = r0; r < kRows; r += 4) {
+        for (int r = r0; r < kRows; r += kStep) {
           uint4* at = reinterpret_cast<uint4*>(dst + r * 128 + (((c & 7) ^ (r & 7)) << 4));
           uint4 v = *at;
           float up = 1.0f;
@@ -381,7 +380,7 @@ paged_tree_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ C
             };
             float mx = fmaxf(fmaxf(top(v.x), top(v.y)), fmaxf(top(v.z), top(v.w)));
 #pragma unroll
-            for (int o = 8; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+            for (int o = kLanes / 2; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
             int e = 0;
             if (mx > 0.0f) e = min(max(14 - ((int)(__float_as_uint(mx) >> 23) - 127), -100), 100);
             up = pow2f(e);
@@ -569,13 +568,13 @@ paged_tree_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ C
           uint8_t* vrow = smem + L::V0 + st * TILE + rt * 128;
           if (!exists) {
 #pragma unroll 4
-            for (int k = 0; k < 16; ++k)
+            for (int k = 0; k < kD / 8; ++k)
               *reinterpret_cast<uint4*>(vrow + (k >> 3) * BLK + (k & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
           } else if (t >= u.s.prefix) {
             constexpr uint32_t kExp = std::is_same<QT, bf16>::value ? 0x7f80u : 0x7c00u;
             bool sick = false;
 #pragma unroll 2
-            for (int k = 0; k < 16; ++k) {
+            for (int k = 0; k < kD / 8; ++k) {
               uint4* at = reinterpret_cast<uint4*>(vrow + (k >> 3) * BLK + (k & 7) * 16);
               uint4 v = *at;
               bool here = clear_sick(v.x, kExp);
@@ -622,18 +621,18 @@ paged_tree_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ C
         const int slot = slot_of(u, blockIdx.x);
         float inv = 1.0f;
         if (slot < 0) inv = Ls == 0.0f ? (any ? NAN : 0.0f) : 1.0f / Ls;
-        QT* dst = reinterpret_cast<QT*>(p.out) + qrow * p.o_st + (int64_t)head * p.o_sh + stream * 64;
-        float* part = p.part_acc + ((int64_t)(slot < 0 ? 0 : slot) * kRows + rt) * kD + stream * 64;
+        QT* dst = reinterpret_cast<QT*>(p.out) + qrow * p.o_st + (int64_t)head * p.o_sh + stream * (kD / 2);
+        float* part = p.part_acc + ((int64_t)(slot < 0 ? 0 : slot) * kRows + rt) * kD + stream * (kD / 2);
         const bool sick = sick_s[unit % kSickSlots] == (int)unit + 1;
 #pragma unroll 1
-        for (int c = 0; c < 2; ++c) {
+        for (int c = 0; c < kD / 64; ++c) {
           float v[32];
-          tmem_ld32(oa + stream * 64 + 32 * c, v);
+          tmem_ld32(oa + stream * (kD / 2) + 32 * c, v);
 #pragma unroll
           for (int e = 0; e < 32; ++e) v[e] *= a0;
           if (both) {
             float y[32];
-            tmem_ld32(oa + kD + stream * 64 + 32 * c, y);
+            tmem_ld32(oa + kD + stream * (kD / 2) + 32 * c, y);
 #pragma unroll
             for (int e = 0; e < 32; ++e) v[e] = fmaf(y[e], a1, v[e]);
           }
@@ -656,10 +655,10 @@ paged_tree_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ C
             const int64_t page = load_page(p, u.b, t >> bs_log2);
             if (page < 0 || !(visible32(u.s, mask_row, mask0, p.mask_words, t) & 1u)) continue;
             const int64_t row = (page * p.block_size + (t & (p.block_size - 1))) * p.num_kv_heads + u.kvh;
-            const CT* vr = reinterpret_cast<const CT*>(p.v_cache) + row * kD + stream * 64;
+            const CT* vr = reinterpret_cast<const CT*>(p.v_cache) + row * kD + stream * (kD / 2);
             const float f = kTok ? __ldg(p.v_scales + row) : 1.0f;
 #pragma unroll 1
-            for (int e = 0; e < 64; ++e) {
+            for (int e = 0; e < kD / 2; ++e) {
               const float x2 = to_f32(vr[e]) * f;
               if (isfinite(x2)) continue;
               if (slot < 0) dst[e] = from_f32<QT>(to_f32(dst[e]) + x2);
@@ -697,11 +696,12 @@ paged_tree_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ C
     auto convert = [&](const uint8_t* src, uint8_t* dst, bool valid, bool node) -> bool {
       bool sick = false;
       uint8_t* drow = dst + r * 128;
-      uint4 raw[8];  // all loads first: a store in between would hold the next one back
+      uint4 raw[kD / 16];  // all loads first: a store in between would hold the next one back
+      const int turn = kD == 128 ? r & 7 : (r >> 1) & 3;  // the swizzle of 128- and of 64-byte rows
 #pragma unroll
-      for (int c = 0; c < 8; ++c) raw[c] = *reinterpret_cast<const uint4*>(src + r * 128 + ((c ^ (r & 7)) << 4));
+      for (int c = 0; c < kD / 16; ++c) raw[c] = *reinterpret_cast<const uint4*>(src + r * kD + ((c ^ turn) << 4));
 #pragma unroll
-      for (int c = 0; c < 8; ++c) {
+      for (int c = 0; c < kD / 16; ++c) {
         uint32_t h[8];
         if (!valid) raw[c] = make_uint4(0u, 0u, 0u, 0u);
         to_f16x16<CT>(raw[c], h);
@@ -742,13 +742,13 @@ paged_tree_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ C
         next_e = tok_entry(t + 3 * kTile);
         const bool node = t >= u.s.prefix;
         if (!(ok = wait(&rfull[rs], k / kRS) && wait(&kempty[st], k / kKS + 1))) break;
-        const uint8_t* raw = smem + L::R0 + rs * 2 * BLK;
+        const uint8_t* raw = smem + L::R0 + rs * 2 * L::RAW;
         convert(raw, smem + L::K0 + st * TILE, row >= 0, false);
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&kfull[st]);
         if (!(ok = wait(&vempty[sv], k / kVS + 1))) break;  // PV of tile k - 2 is done, and its scales are read
-        bool sick = convert(raw + BLK, smem + L::V0 + sv * TILE, row >= 0, node);
+        bool sick = convert(raw + L::RAW, smem + L::V0 + sv * TILE, row >= 0, node);
         if constexpr (kTok) {
           // P takes the token's V scale times 2^-vexp: a power of two that follows the largest
           // scale of a tile, moved only when that grows past it or falls 4 binades below
@@ -804,15 +804,15 @@ EncodeTiledFn encode_fn() {  // resolved once (thread-safe static initialisation
   return fn;
 }
 
-template <typename QT, typename CT, bool kTok>
+template <typename QT, typename CT, bool kTok, int kD>
 int launch(const Params& p, int cache_dtype, int ctas, cudaStream_t stream) {
   constexpr bool kByte = sizeof(CT) == 1;
-  using L = Layout<kByte, kTok>;
-  // rows of the map = slots of the cache, each the kv heads' values; boxes of 128 bytes x one
-  // page (or 128 tokens of it)
+  using L = Layout<kByte, kTok, kD>;
+  // rows of the map = slots of the cache, each the kv heads' values; boxes of 128 bytes (8-bit
+  // rows of 64: 64 bytes) x one page (or 128 tokens of it)
   const cuuint64_t dims[2] = {(cuuint64_t)p.num_kv_heads * kD, (cuuint64_t)p.num_blocks * (cuuint64_t)p.block_size};
   const cuuint64_t strides[1] = {(cuuint64_t)p.num_kv_heads * kD * sizeof(CT)};
-  const cuuint32_t box[2] = {kByte ? 128u : 64u, (cuuint32_t)(p.block_size < kTile ? p.block_size : kTile)};
+  const cuuint32_t box[2] = {kByte ? (cuuint32_t)kD : 64u, (cuuint32_t)(p.block_size < kTile ? p.block_size : kTile)};
   const cuuint32_t estr[2] = {1, 1};
   const CUtensorMapDataType dt = kByte ? CU_TENSOR_MAP_DATA_TYPE_UINT8
                                        : (cache_dtype == MKV_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
@@ -820,30 +820,31 @@ int launch(const Params& p, int cache_dtype, int ctas, cudaStream_t stream) {
   CUtensorMap maps[2];
   for (int i = 0; i < 2; ++i) {
     const CUresult r = encode_fn()(&maps[i], dt, 2, const_cast<uint8_t*>(i ? p.v_cache : p.k_cache), dims, strides, box,
-                                   estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                                   estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                                   kByte && kD == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
                                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) return set_error(MKV_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
   }
-  const int st = ensure_dynamic_smem((const void*)paged_tree_tc_kernel<QT, CT, kTok>, L::BYTES,
+  const int st = ensure_dynamic_smem((const void*)paged_tree_tc_kernel<QT, CT, kTok, kD>, L::BYTES,
                                      "cudaFuncSetAttribute(paged_tree_tc smem)");
   if (st != MKV_OK) return st;
-  paged_tree_tc_kernel<QT, CT, kTok><<<ctas, L::kThreads, L::BYTES, stream>>>(p, maps[0], maps[1]);
+  paged_tree_tc_kernel<QT, CT, kTok, kD><<<ctas, L::kThreads, L::BYTES, stream>>>(p, maps[0], maps[1]);
   return cuda_status(cudaGetLastError(), "paged_tree_tc launch");
 }
 
-template <typename QT>
+template <typename QT, int kD>
 int launch_for(const Params& p, int cache_dtype, int ctas, cudaStream_t stream) {
   if (cache_dtype == MKV_DTYPE_FP8_E4M3)
-    return p.k_scales ? launch<QT, fp8, true>(p, cache_dtype, ctas, stream)
-                      : launch<QT, fp8, false>(p, cache_dtype, ctas, stream);
-  if (cache_dtype == MKV_DTYPE_INT8) return launch<QT, int8_t, true>(p, cache_dtype, ctas, stream);
-  return launch<QT, QT, false>(p, cache_dtype, ctas, stream);
+    return p.k_scales ? launch<QT, fp8, true, kD>(p, cache_dtype, ctas, stream)
+                      : launch<QT, fp8, false, kD>(p, cache_dtype, ctas, stream);
+  if (cache_dtype == MKV_DTYPE_INT8) return launch<QT, int8_t, true, kD>(p, cache_dtype, ctas, stream);
+  return launch<QT, QT, false, kD>(p, cache_dtype, ctas, stream);
 }
 
 }  // namespace
 
 bool tc_supported(const Params& p, int q_dtype, int cache_dtype) {
-  if (p.head_dim != kD || (q_dtype != MKV_DTYPE_BF16 && q_dtype != MKV_DTYPE_F16)) return false;
+  if ((p.head_dim != 64 && p.head_dim != 128) || (q_dtype != MKV_DTYPE_BF16 && q_dtype != MKV_DTYPE_F16)) return false;
   if (p.block_size < 8 || (p.block_size & (p.block_size - 1)) != 0) return false;
   if (p.num_blocks <= 0 || p.num_blocks * p.block_size > 0x7fffffffll) return false;  // TMA coordinates
   // 16-byte loads of query rows and stores of output rows
@@ -854,8 +855,11 @@ bool tc_supported(const Params& p, int q_dtype, int cache_dtype) {
 }
 
 int launch_tc(const Params& p, int q_dtype, int cache_dtype, int ctas, cudaStream_t stream) {
-  return q_dtype == MKV_DTYPE_BF16 ? launch_for<bf16>(p, cache_dtype, ctas, stream)
-                                   : launch_for<f16>(p, cache_dtype, ctas, stream);
+  if (p.head_dim == 64)
+    return q_dtype == MKV_DTYPE_BF16 ? launch_for<bf16, 64>(p, cache_dtype, ctas, stream)
+                                     : launch_for<f16, 64>(p, cache_dtype, ctas, stream);
+  return q_dtype == MKV_DTYPE_BF16 ? launch_for<bf16, 128>(p, cache_dtype, ctas, stream)
+                                   : launch_for<f16, 128>(p, cache_dtype, ctas, stream);
 }
 
 }  // namespace tree

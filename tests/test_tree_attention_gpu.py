@@ -149,15 +149,17 @@ def test_types_and_heads(attn, dtype, mode, H, KVH, D):
     ([0], [1]), ([1], [1]), ([15], [1]), ([16], [2]), ([63], [1]), ([64], [1]), ([127], [3]), ([128], [64]),
     ([0, 0, 0], [0, 1, 0]), ([5, 1000, 0, 130], [3, 1, 64, 33]), ([1100], [65]), ([61], [130]), ([0], [97]),
     ([2000] * 3 + [1] * 9, [1] * 12)])
-def test_lengths(attn, mode, prefix, nodes):
-    c = Case(2, prefix, nodes, 8, 2, 128, 16, BF16, mode)
+@pytest.mark.parametrize("D", [64, 128])
+def test_lengths(attn, mode, prefix, nodes, D):
+    c = Case(2, prefix, nodes, 8, 2, D, 16, BF16, mode)
     c.check(c.run(attn))
 
 
 @pytest.mark.parametrize("BS", [1, 7, 8, 16, 48, 64, 128, 256])
-@pytest.mark.parametrize("dtype,mode", [(BF16, "auto"), (F16, "fp8_per_token_head")])
-def test_page_sizes(attn, BS, dtype, mode):
-    c = Case(3, [300, 7, 129], [20, 3, 40], 8, 2, 128, BS, dtype, mode)
+@pytest.mark.parametrize("dtype,mode", [(BF16, "auto"), (F16, "fp8_per_token_head"), (BF16, "int8_per_token_head")])
+@pytest.mark.parametrize("D", [64, 128])
+def test_page_sizes(attn, BS, dtype, mode, D):
+    c = Case(3, [300, 7, 129], [20, 3, 40], 8, 2, D, BS, dtype, mode)
     c.check(c.run(attn))
 
 
@@ -170,6 +172,7 @@ def test_other_head_dims(attn, D, dtype, mode):
 
 @pytest.mark.parametrize("H,KVH", [(7, 1), (10, 2), (32, 1), (160, 1), (3, 3)])
 def test_groups(attn, H, KVH):
+    """Also groups that do not divide the row tile, and rows beyond one tile."""
     c = Case(5, [210, 40], [13, 30], H, KVH, 128, 16, BF16)
     c.check(c.run(attn))
 
@@ -192,14 +195,15 @@ def test_any_mask(attn, dtype, mode):
 @pytest.mark.parametrize("dtype,mode", [(BF16, "auto"), (F16, "auto"), (F32, "auto"), (BF16, "fp8_per_tensor"),
                                         (BF16, "fp8_per_token_head"), (F16, "int8_per_token_head")])
 @pytest.mark.parametrize("prefix", [0, 40, 120, 700])
-def test_hidden_nodes_may_hold_anything(attn, dtype, mode, prefix):
+@pytest.mark.parametrize("D", [64, 128])
+def test_hidden_nodes_may_hold_anything(attn, dtype, mode, prefix, D):
     """A drafted branch that overflowed reaches only the rows that see it."""
     n, sick = 12, 5
     visible = [[{0, j} for j in range(n)]]
     for j in range(n):
         if j != sick:
             visible[0][j].discard(sick)
-    c = Case(7, [prefix], [n], 8, 2, 128, 16, dtype, mode, visible=visible)
+    c = Case(7, [prefix], [n], 8, 2, D, 16, dtype, mode, visible=visible)
     t = prefix + sick
     page, at = int(c.bt[0, t // 16]), t % 16
     if mode == "int8_per_token_head":
@@ -296,12 +300,13 @@ def test_rows_of_no_sequence_are_left(attn):
 
 @pytest.mark.parametrize("dtype,mode", [(BF16, "auto"), (BF16, "fp8_per_tensor"), (F16, "int8_per_token_head")])
 @pytest.mark.parametrize("nodes", [1, 20])
-def test_sharp_and_flat_scores(attn, dtype, mode, nodes):
+@pytest.mark.parametrize("D", [64, 128])
+def test_sharp_and_flat_scores(attn, dtype, mode, nodes, D):
     """Queries 30 times as large (weights down to nothing), and all keys equal (all weights
     equal, values with a common offset)."""
-    c = Case(14, [1500, 3], [nodes, nodes], 8, 2, 128, 64, dtype, mode, spread=30.0)
+    c = Case(14, [1500, 3], [nodes, nodes], 8, 2, D, 64, dtype, mode, spread=30.0)
     c.check(c.run(attn))
-    c = Case(15, [1500, 3], [nodes, nodes], 8, 2, 128, 64, dtype, mode, spread=0.0, offset=2.0)
+    c = Case(15, [1500, 3], [nodes, nodes], 8, 2, D, 64, dtype, mode, spread=0.0, offset=2.0)
     c.check(c.run(attn))
 
 
@@ -338,6 +343,37 @@ def test_pages_past_32_bits(attn):
     c.k, c.v = k[pages], v[pages]  # the oracle on the three pages alone
     c.bt = torch.tensor([[0, 1, 2]], dtype=torch.int32, device=DEV)
     c.check(got)
+
+
+def test_negative_and_zero_scales(attn):
+    """A score scale below 0 prefers the least alike; 0 makes every weight equal."""
+    for dtype, mode in ((BF16, "auto"), (F16, "fp8_per_tensor"), (BF16, "int8_per_token_head"), (F32, "auto")):
+        for scale in (-0.09, 0.0):
+            c = Case(22, [200, 3], [9, 20], 8, 2, 128, 16, dtype, mode)
+            c.scale = scale
+            c.check(c.run(attn))
+
+
+@pytest.mark.parametrize("size", [1e-6, 1e4])
+@pytest.mark.parametrize("mode", ["fp8_per_tensor", "int8_per_token_head", "fp8_per_token_head"])
+def test_sizes_of_queries_and_values(attn, size, mode):
+    """Queries and value scales far from 1 (f16 operands hold only so much)."""
+    c = Case(23, [300, 40], [12, 3], 8, 2, 128, 16, BF16, mode)
+    c.q = (c.q.float() * size).to(BF16)
+    c.ks = c.ks / size
+    c.vs = c.vs * size
+    c.check(c.run(attn))
+
+
+def test_value_scales_of_every_size(attn):
+    """Per-(token, head) value scales that differ by 2^20 within and between tiles, up and down."""
+    c = Case(24, [1000], [30], 8, 2, 128, 16, BF16, "int8_per_token_head")
+    g = torch.Generator(device=DEV).manual_seed(24)
+    c.vs = c.vs * torch.exp2(torch.randint(-10, 11, c.vs.shape, generator=g, device=DEV).float())
+    at = c.bt[0].long()
+    c.vs[at[:20]] *= 2.0 ** 12
+    c.vs[at[40:50]] *= 2.0 ** -12
+    c.check(c.run(attn))
 
 
 @pytest.mark.parametrize("dtype,mode,nodes", [(BF16, "auto", 3), (BF16, "auto", 40), (BF16, "fp8_per_tensor", 8),
