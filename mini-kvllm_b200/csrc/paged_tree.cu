@@ -397,6 +397,7 @@ extern "C" int mkv_paged_tree_attention(
   const tree::Plan plan = tree::tc_supported(p, q_dtype, cache_dtype)
                               ? tree::Plan{true, tree::kTcRows, kNumSMs}
                               : tree::Plan{false, tree::kGRows, tree::kGCtas};
+  p.unit_cost = plan.tc ? (cache_dtype == q_dtype ? 4 : 2) : 0;
   const tree::Workspace w = tree::workspace(plan.ctas, plan.rows, head_dim);
   p.part_acc = (float*)((char*)workspace + w.acc);
   p.part_ml = (float2*)((char*)workspace + w.ml);

@@ -25,6 +25,7 @@ struct Params {
   int mask_words;
   int num_seqs, num_heads, num_kv_heads, head_dim, group;
   int64_t total_q;
+  int unit_cost;  // of the schedule, in token tiles
   float qk_scale_log2;
   const float* k_scale;   // per-tensor scales of e4m3 pages, or null
   const float* v_scale;
@@ -119,13 +120,14 @@ __device__ __forceinline__ uint32_t visible32(const Seq& s, const uint64_t* mask
 
 // ---------------------------------------------------------------- work schedule
 // Work items are (sequence, kv head, tile of RT query rows, tile of KT tokens), in this
-// order; a unit is a run of all token tiles of one row tile. CTA c of n takes items
-// [c W / n, (c + 1) W / n): equal work whatever the lengths, known on the device alone. A
-// unit that ends inside a CTA's share is written there whole; the parts of a unit that
-// crosses shares go to partial slots (2 c + 1: the part that starts a unit, 2 c: any later
-// one) and are joined by the combine kernel, which takes its orders from desc[c]: the
-// first CTA that continues a unit gives the number of its parts, its kv head and first row,
-// and the rows and the first query row of its sequence.
+// order; a unit is a run of all token tiles of one row tile, followed by unit_cost items that
+// stand for what a unit costs besides its tiles. CTA c of n takes items
+// [c W / n, (c + 1) W / n): equal work whatever the lengths, known on the device alone. A unit
+// that ends inside a CTA's share is written there whole; the parts of a unit that crosses
+// shares go to partial slots (2 c + 1: the part that starts a unit, 2 c: any later one) and are
+// joined by the combine kernel, which takes its orders from desc[c]: the first CTA that
+// continues a unit gives the number of its parts, its kv head and first row, and the rows and
+// the first query row of its sequence.
 struct Unit {
   int b, kvh, mt;     // sequence, kv head, row tile
   int k0, k1, tiles;  // token tiles taken here, and of the whole unit
@@ -142,7 +144,7 @@ template <int RT, int KT>
 __device__ __forceinline__ int64_t items_of(const Params& p, const Seq& s, int& mt, int& kt) {
   mt = (int)(((int64_t)s.nodes * p.group + RT - 1) / RT);
   kt = max(1, (s.len + KT - 1) / KT);
-  return (int64_t)p.num_kv_heads * mt * kt;
+  return (int64_t)p.num_kv_heads * mt * (kt + p.unit_cost);
 }
 
 struct Walk {
@@ -215,12 +217,16 @@ __device__ bool begin(const Params& p, int c, int n, long long* red, Walk& w) {
   const int64_t off = found[1];
   w.s = load_seq(p, w.b);
   items_of<RT, KT>(p, w.s, w.mts, w.kts);
-  const int64_t i = quot(off, w.kts);
-  w.k = (int)(off - i * w.kts);
+  const int per = w.kts + p.unit_cost;
+  const int64_t i = quot(off, per);
+  w.k = (int)(off - i * per);
   w.kvh = (int)quot(i, w.mts);
   w.mt = (int)(i - (int64_t)w.kvh * w.mts);
   const int64_t unit0 = s0 - w.k;  // first item of the unit that s0 lies in
-  if (tid == 0 && w.k > 0 && quot((int64_t)(c - 1) * total, n) <= unit0) {
+  if (w.k >= w.kts) {  // behind its tiles
+    w.left -= per - w.k;
+    w.k = w.kts;
+  } else if (tid == 0 && w.k > 0 && quot((int64_t)(c - 1) * total, n) <= unit0) {
     // this CTA is the first to continue the unit: parts from CTA c - 1 to the one holding its last item
     const int64_t last = quot((unit0 + w.kts) * n + total - 1, total) - 1;
     p.desc[2 * c + 1] = make_int4((int)(w.s.q0 >> 32), (int)w.s.q0, 0, 0);
@@ -255,6 +261,7 @@ __device__ __forceinline__ bool next(const Params& p, Walk& w, Unit& u) {
   u.tiles = w.kts;
   u.k1 = (int)min((int64_t)w.kts, w.k + w.left);
   w.left -= u.k1 - u.k0;
+  if (u.k1 == w.kts) w.left -= p.unit_cost;
   w.k = u.k1;
   return true;
 }

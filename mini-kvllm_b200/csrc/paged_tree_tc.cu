@@ -176,6 +176,7 @@ paged_tree_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ C
   tc_fence_before_sync();
   __syncthreads();
   tc_fence_after_sync();
+  pdl_trigger();  // the combine kernel may be set up (it waits for this one's end)
   const uint32_t tmem = *tmem_base_s;
   if (!work) {
     if (warp == 1) tmem_dealloc(tmem, kTmemCols);

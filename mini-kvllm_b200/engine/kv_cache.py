@@ -238,20 +238,23 @@ def _tree_args(fn: str, parents, cu_seqlens_q, prefix_lens, block_tables, block_
     parents = _indices(fn, "parents", parents, 1)
     cu = _indices(fn, "cu_seqlens_q", cu_seqlens_q, 1)
     prefix = _indices(fn, "prefix_lens", prefix_lens, 1)
-    if block_tables.dtype not in _INDEX or block_tables.dim() != 2:
+    tables = block_tables
+    tt = _INDEX.get(tables.dtype)
+    if tt is None or tables.dim() != 2:
         raise ValueError(f"{fn}: block_tables must be a two-dimensional int32 or int64 tensor")
-    if block_tables.stride(1) != 1:
-        block_tables = block_tables.contiguous()
+    stride = tables.stride()
+    if stride[1] != 1:
+        tables = tables.contiguous()
+        stride = tables.stride()
+    rows, width = tables.shape
     B = prefix.numel()
-    if cu.numel() != B + 1 or block_tables.shape[0] < B:
+    if cu.numel() != B + 1 or rows < B:
         raise ValueError(f"{fn}: cu_seqlens_q/block_tables do not match {B} sequences")
     if block_size <= 0:
         raise ValueError(f"{fn}: block_size must be positive")
-    args = (parents.data_ptr(), _INDEX[parents.dtype], cu.data_ptr(), _INDEX[cu.dtype],
-            prefix.data_ptr(), _INDEX[prefix.dtype], block_tables.data_ptr(),
-            _INDEX[block_tables.dtype], block_tables.stride(0), block_tables.shape[1], block_size, B,
-            parents.numel())
-    return (parents, cu, prefix, block_tables), args
+    return (parents, cu, prefix, tables), (
+        parents.data_ptr(), _INDEX[parents.dtype], cu.data_ptr(), _INDEX[cu.dtype], prefix.data_ptr(),
+        _INDEX[prefix.dtype], tables.data_ptr(), tt, stride[0], width, block_size, B, parents.numel())
 
 
 def tree_metadata(parents: torch.Tensor, cu_seqlens_q: torch.Tensor, prefix_lens: torch.Tensor,
@@ -268,11 +271,11 @@ def tree_metadata(parents: torch.Tensor, cu_seqlens_q: torch.Tensor, prefix_lens
         raise ValueError(f"{fn}: max_nodes must be 1 to 1024 (got {max_nodes})")
     idx = _device_index(fn, parents, cu_seqlens_q, prefix_lens, block_tables)
     keep, args = _tree_args(fn, parents, cu_seqlens_q, prefix_lens, block_tables, block_size)
-    B, total, words = args[-2], args[-1], (max_nodes + 63) // 64
-    slots = parents.new_empty(total, dtype=torch.int64)
-    lens = parents.new_empty(B, dtype=torch.int64)
-    positions = parents.new_empty(total, dtype=torch.int64)
-    mask = parents.new_empty((total, words), dtype=torch.int64)
+    B, total, words, dev = args[-2], args[-1], (max_nodes + 63) // 64, parents.device
+    slots = torch.empty(total, dtype=torch.int64, device=dev)
+    lens = torch.empty(B, dtype=torch.int64, device=dev)
+    positions = torch.empty(total, dtype=torch.int64, device=dev)
+    mask = torch.empty(total, words, dtype=torch.int64, device=dev)
     st = _call_packed(_lib.load(), idx, _lib.CALL_TREE_METADATA, _lib.PACK_TREE_METADATA, args + (
         words, slots.data_ptr(), lens.data_ptr(), positions.data_ptr(), mask.data_ptr(), 0))
     if st:
@@ -298,10 +301,12 @@ def tree_accept(draft_tokens: torch.Tensor, target_tokens: torch.Tensor, parents
         raise ValueError(f"{fn}: draft_tokens and target_tokens must be {total} tokens each, of one dtype")
     if max_path < 1:
         raise ValueError(f"{fn}: max_path must be at least 1 (got {max_path})")
-    tokens, src, dst = parents.new_empty((3, B, max_path), dtype=torch.int64).unbind(0)
-    nodes = parents.new_empty((B, max_path), dtype=torch.int32)
-    count = parents.new_empty(B, dtype=torch.int32)
-    lens = parents.new_empty(B, dtype=torch.int64)
+    dev = parents.device
+    tokens = torch.empty(B, max_path, dtype=torch.int64, device=dev)
+    src, dst = torch.empty_like(tokens), torch.empty_like(tokens)
+    nodes = torch.empty(B, max_path, dtype=torch.int32, device=dev)
+    count = torch.empty(B, dtype=torch.int32, device=dev)
+    lens = torch.empty(B, dtype=torch.int64, device=dev)
     st = _call_packed(_lib.load(), idx, _lib.CALL_TREE_ACCEPT, _lib.PACK_TREE_ACCEPT, (
         draft.data_ptr(), target.data_ptr(), _INDEX[draft.dtype]) + args + (
         max_path, count.data_ptr(), nodes.data_ptr(), tokens.data_ptr(), lens.data_ptr(), src.data_ptr(),

@@ -637,7 +637,10 @@ def paged_attention_tree(query: torch.Tensor, k_cache: torch.Tensor, v_cache: to
         _check_row_scales(fn, k_scale, v_scale, num_blocks, block_size, num_kv_heads)
         kps, vps = k_scale.data_ptr(), v_scale.data_ptr()
         cache_code = _DTYPES[want]
-    output = out if out is not None else query.new_empty(query.shape)
+    if out is not None:
+        output = out
+    else:
+        output = torch.empty_like(query) if query.is_contiguous() else query.new_empty(query.shape)
     if total_q == 0 or num_seqs == 0:
         return output
     qs = query.stride()
