@@ -88,17 +88,25 @@ __device__ __forceinline__ void to_f16x16(const uint4 raw, uint32_t (&h)[8]) {
   }
 }
 
-// Clears the infinities and NaN of a pair of 16-bit values (kExp: the type's exponent bits);
-// true when there were any.
-__device__ __forceinline__ bool clear_sick(uint32_t& w, uint32_t exp) {
+// Clears the infinities and NaN of a row of 16-bit values in a tile (kExp: the type's exponent
+// bits; `bytes` of them from `row`, the other 64 columns BLK further on); true when there were
+// any. Out of line, like wait_on: few tiles hold nodes.
+template <uint32_t kExp>
+__device__ __noinline__ bool clear_sick(uint8_t* row, int bytes) {
   bool sick = false;
-  if ((w & exp) == exp) {
-    w &= 0xffff0000u;
-    sick = true;
-  }
-  if ((w >> 16 & exp) == exp) {
-    w &= 0x0000ffffu;
-    sick = true;
+#pragma unroll 1
+  for (int c = 0; c < bytes; c += 16) {
+    uint4* at = reinterpret_cast<uint4*>(row + (c >> 7) * BLK + (c & 127));
+    uint32_t w[4] = {at->x, at->y, at->z, at->w};
+    bool here = false;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const uint32_t keep = ((w[e] & kExp) == kExp ? 0u : 0x0000ffffu) | ((w[e] >> 16 & kExp) == kExp ? 0u : 0xffff0000u);
+      here |= keep != 0xffffffffu;
+      w[e] &= keep;
+    }
+    if (here) *at = make_uint4(w[0], w[1], w[2], w[3]);
+    sick |= here;
   }
   return sick;
 }
@@ -199,7 +207,7 @@ paged_tree_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ C
     return e;
   };
   auto seg_page = [&](const Unit& u, int t, Entry e) -> int64_t { return seg_in(u, t) ? page_of(p, e) : -1; };
-  Unit u;
+  Unit u = {};
   uint32_t g = 0;     // tiles of this CTA before the unit's
   uint32_t unit = 0;  // units before this one
   bool ok = true;
@@ -211,16 +219,13 @@ paged_tree_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ C
       tma_prefetch_map(&vmap);
     }
     uint32_t nk = 0, nv = 0;  // K and V tiles issued (8-bit: nk counts both)
-    // loads the rows of tile t that exist; the rest of the stage keeps what it held
+    // loads the rows of tile t that exist, each lane its own segment (with pages of 16 tokens a tile is
+    // 16 to 32 loads); the rest of the stage keeps what it held
     auto load = [&](const CUtensorMap* map, int t, int64_t page, uint32_t dst, uint64_t* bar) {
-#pragma unroll 1
-      for (int sgi = 0; sgi < nseg; ++sgi) {
-        const int64_t pg = __shfl_sync(0xffffffffu, page, sgi);
-        if (lane == 0 && pg >= 0) {
-          const int y = (int)(pg * p.block_size) + ((t * kTile + sgi * seg_rows) & (p.block_size - 1));
-          tma_load_2d(dst + sgi * seg_rows * (kByte ? kD : 128), map, u.kvh * kD, y, bar);
-          if constexpr (!kByte && kD == 128) tma_load_2d(dst + BLK + sgi * seg_rows * 128, map, u.kvh * kD + 64, y, bar);
-        }
+      if (page >= 0) {
+        const int y = (int)(page * p.block_size) + ((t * kTile + lane * seg_rows) & (p.block_size - 1));
+        tma_load_2d(dst + lane * seg_rows * (kByte ? kD : 128), map, u.kvh * kD, y, bar);
+        if constexpr (!kByte && kD == 128) tma_load_2d(dst + BLK + lane * seg_rows * 128, map, u.kvh * kD + 64, y, bar);
       }
       __syncwarp();
     };
@@ -572,19 +577,7 @@ paged_tree_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ C
             for (int k = 0; k < kD / 8; ++k)
               *reinterpret_cast<uint4*>(vrow + (k >> 3) * BLK + (k & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
           } else if (t >= u.s.prefix) {
-            constexpr uint32_t kExp = std::is_same<QT, bf16>::value ? 0x7f80u : 0x7c00u;
-            bool sick = false;
-#pragma unroll 2
-            for (int k = 0; k < kD / 8; ++k) {
-              uint4* at = reinterpret_cast<uint4*>(vrow + (k >> 3) * BLK + (k & 7) * 16);
-              uint4 v = *at;
-              bool here = clear_sick(v.x, kExp);
-              here |= clear_sick(v.y, kExp);
-              here |= clear_sick(v.z, kExp);
-              here |= clear_sick(v.w, kExp);
-              if (here) *at = v;
-              sick |= here;
-            }
+            const bool sick = clear_sick<std::is_same<QT, bf16>::value ? 0x7f80u : 0x7c00u>(vrow, kD * 2);
             if (sick) sick_s[unit % kSickSlots] = (int)unit + 1;
           }
           fence_proxy_async_smem();
@@ -694,8 +687,7 @@ paged_tree_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ C
       const int64_t page = t < u.s.len ? page_of(p, e) : -1;
       return page < 0 ? -1 : (page * p.block_size + (t & (p.block_size - 1))) * p.num_kv_heads + u.kvh;
     };
-    auto convert = [&](const uint8_t* src, uint8_t* dst, bool valid, bool node) -> bool {
-      bool sick = false;
+    auto convert = [&](const uint8_t* src, uint8_t* dst, bool valid) {
       uint8_t* drow = dst + r * 128;
       uint4 raw[kD / 16];  // all loads first: a store in between would hold the next one back
       const int turn = kD == 128 ? r & 7 : (r >> 1) & 3;  // the swizzle of 128- and of 64-byte rows
@@ -706,15 +698,10 @@ paged_tree_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ C
         uint32_t h[8];
         if (!valid) raw[c] = make_uint4(0u, 0u, 0u, 0u);
         to_f16x16<CT>(raw[c], h);
-        if (node && std::is_same<CT, fp8>::value) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) sick |= clear_sick(h[e], 0x7c00u);
-        }
         const int cc = (c & 3) * 2;  // columns 16c ..: half c / 4, chunks cc and cc + 1
         *reinterpret_cast<uint4*>(drow + (c >> 2) * BLK + ((cc ^ (r & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
         *reinterpret_cast<uint4*>(drow + (c >> 2) * BLK + (((cc + 1) ^ (r & 7)) << 4)) = make_uint4(h[4], h[5], h[6], h[7]);
       }
-      return sick;
     };
 #pragma unroll 1
     while (ok && next<kRows, kTile>(p, walk, u)) {
@@ -742,14 +729,22 @@ paged_tree_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ C
         vs2 = scale_of(p.v_scales, row2);
         next_e = tok_entry(t + 3 * kTile);
         const bool node = t >= u.s.prefix;
-        if (!(ok = wait(&rfull[rs], k / kRS) && wait(&kempty[st], k / kKS + 1))) break;
+        if (!(ok = wait(&rfull[rs], k / kRS))) break;
         const uint8_t* raw = smem + L::R0 + rs * 2 * L::RAW;
-        convert(raw, smem + L::K0 + st * TILE, row >= 0, false);
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&kfull[st]);
-        if (!(ok = wait(&vempty[sv], k / kVS + 1))) break;  // PV of tile k - 2 is done, and its scales are read
-        bool sick = convert(raw + L::RAW, smem + L::V0 + sv * TILE, row >= 0, node);
+#pragma unroll 1
+        for (int v = 0; v < 2; ++v) {  // K, then V (once PV of tile k - 2 is done, and its scales are read)
+          if (!(ok = v == 0 ? wait(&kempty[st], k / kKS + 1) : wait(&vempty[sv], k / kVS + 1))) break;
+          convert(raw + v * L::RAW, smem + (v == 0 ? L::K0 + st * TILE : L::V0 + sv * TILE), row >= 0);
+          if (v == 0) {
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&kfull[st]);
+          }
+        }
+        if (!ok) break;
+        bool sick = false;
+        if (std::is_same<CT, fp8>::value && node && row >= 0)
+          sick = clear_sick<0x7c00u>(smem + L::V0 + sv * TILE + r * 128, kD * 2);
         if constexpr (kTok) {
           // P takes the token's V scale times 2^-vexp: a power of two that follows the largest
           // scale of a tile, moved only when that grows past it or falls 4 binades below
