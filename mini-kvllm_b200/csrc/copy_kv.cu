@@ -6,21 +6,24 @@
 // A copy moves `unit` bytes (a page, or one token's row of all kv heads) from unit src[i]
 // to unit dst[i] of every plane (layer x {K, V}, and their scales). Copies are applied in
 // order i = 0, 1, ..., each seeing what the earlier ones wrote, whatever the indices
-// repeat: a thread owns one 16-byte column of the unit and makes all copies of its column
-// itself, so no other thread ever touches those bytes and program order is the only order
-// needed. Eight copies are in flight per thread (loads first, then stores); when a copy of
-// the eight reads what an earlier one of them writes, the eight are made one at a time.
+// repeat: a thread owns a 16-byte column of the unit in a few layers and makes all copies of
+// its columns itself, so no other thread ever touches those bytes and program order is the
+// only order needed. Four copies of two layers are in flight per thread (loads first, then
+// stores); when a copy of the four reads what an earlier one of them writes, they are made one
+// at a time.
 //
 // Bound: memory, 2 x unit bytes a copy. The columns of a whole cache (28 layers of 32 KB
-// pages: 114688) with eight 16-byte loads each keep 14 MB in flight, enough to cover the
-// latency of HBM; rows take one group of copies per sequence, groups side by side.
+// pages: 114688) keep 14 MB in flight, enough to cover the latency of HBM, and their threads
+// fit the GPU at once. A group of row copies is one sequence's, groups side by side; there a
+// thread's layers share the reading and checking of the indices.
 #include "mkv_common.cuh"
 
 namespace mkv {
 namespace {
 
 constexpr int kCopyThreads = 128;
-constexpr int kInFlight = 8;
+constexpr int kInFlight = 4;
+constexpr int kCopyCtas = 5;  // resident on an SM
 
 struct CopyParams {
   uint8_t* base[2];      // K and V of layer 0
@@ -32,6 +35,7 @@ struct CopyParams {
   int svec;              // column width of the scales, 16 or 4 bytes (K and V: 16)
   int64_t num_units;
   int num_layers;
+  int per_thread;        // layers that a thread takes
   const void* src;
   const void* dst;
   int i64;
@@ -45,73 +49,115 @@ __device__ __forceinline__ int64_t cp_index(const CopyParams& c, const void* p, 
                : (int64_t)__ldg(reinterpret_cast<const int32_t*>(p) + i);
 }
 
-// Loads and stores in program order (volatile, with a memory clobber): a thread may read
-// what it has written.
-__device__ __forceinline__ uint4 cp_load(const uint8_t* p, uint4) {
-  uint4 r;
-  asm volatile("ld.global.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p) : "memory");
-  return r;
+// Loads and stores where `on`, in program order (volatile, with a memory clobber): a thread
+// may read what it has written. Predicated, not branched around: the loads of a batch stay
+// together.
+__device__ __forceinline__ void cp_load(const uint8_t* p, bool on, uint4& r) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+      "@q ld.global.v4.u32 {%0,%1,%2,%3}, [%4];\n\t}"
+      : "+r"(r.x), "+r"(r.y), "+r"(r.z), "+r"(r.w)
+      : "l"(p), "r"((int)on)
+      : "memory");
 }
-__device__ __forceinline__ uint32_t cp_load(const uint8_t* p, uint32_t) {
-  uint32_t r;
-  asm volatile("ld.global.u32 %0, [%1];" : "=r"(r) : "l"(p) : "memory");
-  return r;
+__device__ __forceinline__ void cp_load(const uint8_t* p, bool on, uint32_t& r) {
+  asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %2, 0;\n\t@q ld.global.u32 %0, [%1];\n\t}"
+               : "+r"(r)
+               : "l"(p), "r"((int)on)
+               : "memory");
 }
-__device__ __forceinline__ void cp_store(uint8_t* p, uint4 v) { st_v4(p, v); }
-__device__ __forceinline__ void cp_store(uint8_t* p, uint32_t v) {
-  asm volatile("st.global.u32 [%0], %1;" ::"l"(p), "r"(v) : "memory");
+__device__ __forceinline__ void cp_store(uint8_t* p, bool on, const uint4& v) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+      "@q st.global.v4.u32 [%0], {%1,%2,%3,%4};\n\t}" ::"l"(p),
+      "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w), "r"((int)on)
+      : "memory");
+}
+__device__ __forceinline__ void cp_store(uint8_t* p, bool on, uint32_t v) {
+  asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %2, 0;\n\t@q st.global.u32 [%0], %1;\n\t}" ::"l"(p), "r"(v),
+               "r"((int)on)
+               : "memory");
 }
 
-// All copies of one column of a group: p points at its bytes in unit 0, T is its type.
-// A negative entry is no copy; one past the cache is skipped.
+// All copies of one column of a group in `layers` layers, `stride` bytes apart: p points at its
+// bytes in unit 0 of the first, T is its type. A negative entry is no copy; one past the cache
+// is skipped.
 template <typename T>
-__device__ __forceinline__ void copy_column(const CopyParams& c, uint8_t* p, int64_t unit, int64_t first) {
+__device__ __forceinline__ void copy_column(const CopyParams& c, uint8_t* p, int64_t stride, int layers,
+                                            int64_t unit, int64_t first) {
+#pragma unroll 1
   for (int i0 = 0; i0 < c.num_copies; i0 += kInFlight) {
     int64_t s[kInFlight], d[kInFlight];
-    bool chained = false;
+    bool chained = false, any = false;
 #pragma unroll
     for (int u = 0; u < kInFlight; ++u) {
       s[u] = d[u] = -1;
       if (i0 + u < c.num_copies) {
         s[u] = cp_index(c, c.src, first + i0 + u);
         d[u] = cp_index(c, c.dst, first + i0 + u);
-        if (s[u] < 0 || d[u] < 0 || s[u] >= c.num_units || d[u] >= c.num_units) s[u] = d[u] = -1;
       }
+      if (s[u] < 0 || d[u] < 0 || s[u] >= c.num_units || d[u] >= c.num_units) s[u] = d[u] = -1;
+      any |= s[u] >= 0;
 #pragma unroll
       for (int w = 0; w < u; ++w) chained |= s[u] >= 0 && s[u] == d[w];
     }
-    T x[kInFlight];
+    if (!any) continue;
+#pragma unroll
+    for (int u = 0; u < kInFlight; ++u) {  // byte offsets from here on
+      if (s[u] >= 0) {
+        s[u] *= unit;
+        d[u] *= unit;
+      }
+    }
+    uint8_t* q = p;
     if (!chained) {
+#pragma unroll 1
+      for (int l = 0; l < layers; l += 2, q += 2 * stride) {
+        const bool two = l + 1 < layers;
+        T x[2][kInFlight] = {};
 #pragma unroll
-      for (int u = 0; u < kInFlight; ++u)
-        if (s[u] >= 0) x[u] = cp_load(p + s[u] * unit, T());
+        for (int u = 0; u < kInFlight; ++u) {
+          cp_load(q + s[u], s[u] >= 0, x[0][u]);
+          cp_load(q + stride + s[u], s[u] >= 0 && two, x[1][u]);
+        }
 #pragma unroll
-      for (int u = 0; u < kInFlight; ++u)
-        if (s[u] >= 0) cp_store(p + d[u] * unit, x[u]);
+        for (int u = 0; u < kInFlight; ++u) {
+          cp_store(q + d[u], s[u] >= 0, x[0][u]);
+          cp_store(q + stride + d[u], s[u] >= 0 && two, x[1][u]);
+        }
+      }
     } else {
+#pragma unroll 1
+      for (int l = 0; l < layers; ++l, q += stride) {
 #pragma unroll
-      for (int u = 0; u < kInFlight; ++u)
-        if (s[u] >= 0) cp_store(p + d[u] * unit, cp_load(p + s[u] * unit, T()));
+        for (int u = 0; u < kInFlight; ++u) {
+          T x = {};
+          cp_load(q + s[u], s[u] >= 0, x);
+          cp_store(q + d[u], s[u] >= 0, x);
+        }
+      }
     }
   }
 }
 
-__global__ void __launch_bounds__(kCopyThreads) copy_units_kernel(const CopyParams c) {
+__global__ void __launch_bounds__(kCopyThreads, kCopyCtas) copy_units_kernel(const __grid_constant__ CopyParams c) {
   const int64_t cols = c.unit / 16, scols = c.sunit ? c.sunit / c.svec : 0;
-  const int64_t planes = 2 * c.num_layers;
+  const int64_t parts = (c.num_layers + c.per_thread - 1) / c.per_thread;  // of the layers
   const int64_t at = (int64_t)blockIdx.x * kCopyThreads + threadIdx.x;
   for (int g = blockIdx.y; g < c.num_groups; g += gridDim.y) {
     const int64_t first = (int64_t)g * c.num_copies;
-    if (at < planes * cols) {
-      const int64_t plane = at / cols, col = at - plane * cols;
-      const int64_t layer = plane >> 1;
-      copy_column<uint4>(c, c.base[plane & 1] + layer * c.plane_stride + col * 16, c.unit, first);
-    } else if (at < planes * (cols + scols)) {
-      const int64_t a = at - planes * cols;
-      const int64_t plane = a / scols, col = a - plane * scols;
-      uint8_t* p = c.sbase[plane & 1] + (plane >> 1) * c.splane_stride + col * c.svec;
-      if (c.svec == 16) copy_column<uint4>(c, p, c.sunit, first);
-      else copy_column<uint32_t>(c, p, c.sunit, first);
+    const bool values = at < 2 * parts * cols;
+    const int64_t a = values ? at : at - 2 * parts * cols;
+    const int64_t n = values ? cols : scols;
+    if (n > 0 && a < 2 * parts * n) {
+      const int64_t part = a / n, col = a - part * n;
+      const int l0 = (int)(part >> 1) * c.per_thread, layers = min(c.per_thread, c.num_layers - l0);
+      if (values)
+        copy_column<uint4>(c, (part & 1 ? c.base[1] : c.base[0]) + l0 * c.plane_stride + col * 16, c.plane_stride, layers, c.unit, first);
+      else if (c.svec == 16)
+        copy_column<uint4>(c, (part & 1 ? c.sbase[1] : c.sbase[0]) + l0 * c.splane_stride + col * 16, c.splane_stride, layers, c.sunit, first);
+      else
+        copy_column<uint32_t>(c, (part & 1 ? c.sbase[1] : c.sbase[0]) + l0 * c.splane_stride + col * 4, c.splane_stride, layers, c.sunit, first);
     }
     if (c.invalid_count != nullptr && blockIdx.x == 0) {
       int bad = 0;
@@ -168,7 +214,15 @@ int copy_units(const char* fn, void* k_cache, void* v_cache, int32_t cache_dtype
   c.num_copies = (int)num_copies;
   c.num_groups = num_groups;
   c.invalid_count = invalid_count;
-  const int64_t columns = 2 * (int64_t)num_layers * (c.unit / 16 + (c.sunit ? c.sunit / c.svec : 0));
+  // layers a thread, at most 8: as many as bring the grid down to what is resident at once (a page copy
+  // in two waves takes 1.5 times as long), and no more: one stream's move of a few rows is bound by
+  // latency and wants a thread for each column, a batch's reads its indices less often this way (44 us
+  // against 92 for 253 sequences of up to 7 moves).
+  const int64_t unit_cols = c.unit / 16 + (c.sunit ? c.sunit / c.svec : 0);
+  const int64_t resident = (int64_t)kNumSMs * kCopyCtas * kCopyThreads;
+  const int64_t waves = (2 * unit_cols * num_layers * (num_groups < 65535 ? num_groups : 65535) + resident - 1) / resident;
+  c.per_thread = (int)(waves < 1 ? 1 : waves > 8 ? 8 : waves);
+  const int64_t columns = 2 * unit_cols * ((num_layers + c.per_thread - 1) / c.per_thread);
   const int64_t ctas = (columns + kCopyThreads - 1) / kCopyThreads;
   if (ctas > 0x7fffffff) return set_error(MKV_ERR_INVALID_ARGUMENT, "%s: bad sizes", fn);
   const dim3 grid((unsigned)ctas, (unsigned)(num_groups < 65535 ? num_groups : 65535));
