@@ -14,7 +14,10 @@
 //
 // Bound: memory, 2 x unit bytes a copy. The columns of a whole cache (28 layers of 32 KB
 // pages: 114688) keep 14 MB in flight, enough to cover the latency of HBM, and their threads
-// fit the GPU at once. A group of row copies is one sequence's, groups side by side; there a
+// fit the GPU at once. Where the columns are few and the pairs many (small pages of one kv
+// head), the pairs are split over CTAs as well, if none of them writes what another one reads or
+// writes: every CTA finds that out for itself, with a hash table of the destinations.
+// A group of row copies is one sequence's, groups side by side; there a
 // thread's layers share the reading and checking of the indices.
 #include "mkv_common.cuh"
 
@@ -24,6 +27,7 @@ namespace {
 constexpr int kCopyThreads = 128;
 constexpr int kInFlight = 4;
 constexpr int kCopyCtas = 5;  // resident on an SM
+constexpr int kSplitPairs = 1024, kHashSlots = 2 * kSplitPairs;  // pairs of a launch that may split them
 
 struct CopyParams {
   uint8_t* base[2];      // K and V of layer 0
@@ -84,15 +88,15 @@ __device__ __forceinline__ void cp_store(uint8_t* p, bool on, uint32_t v) {
 // is skipped.
 template <typename T>
 __device__ __forceinline__ void copy_column(const CopyParams& c, uint8_t* p, int64_t stride, int layers,
-                                            int64_t unit, int64_t first) {
+                                            int64_t unit, int64_t first, int count) {
 #pragma unroll 1
-  for (int i0 = 0; i0 < c.num_copies; i0 += kInFlight) {
+  for (int i0 = 0; i0 < count; i0 += kInFlight) {
     int64_t s[kInFlight], d[kInFlight];
     bool chained = false, any = false;
 #pragma unroll
     for (int u = 0; u < kInFlight; ++u) {
       s[u] = d[u] = -1;
-      if (i0 + u < c.num_copies) {
+      if (i0 + u < count) {
         s[u] = cp_index(c, c.src, first + i0 + u);
         d[u] = cp_index(c, c.dst, first + i0 + u);
       }
@@ -140,12 +144,56 @@ __device__ __forceinline__ void copy_column(const CopyParams& c, uint8_t* p, int
   }
 }
 
+// Whether some pair of c writes a unit that another one reads or writes. Block-collective; the
+// same answer in every block.
+__device__ bool pairs_clash(const CopyParams& c) {
+  __shared__ long long table[kHashSlots];
+  __shared__ int clash;
+  for (int i = threadIdx.x; i < kHashSlots; i += kCopyThreads) table[i] = -1;
+  if (threadIdx.x == 0) clash = 0;
+  __syncthreads();
+  auto slot = [](int64_t v) { return (uint32_t)((uint64_t)v * 0x9E3779B97F4A7C15ull >> 53); };  // 11 bits
+  static_assert(kHashSlots == 2048, "slot() has 11 bits");
+#pragma unroll 1
+  for (int pass = 0; pass < 2; ++pass) {  // enter the destinations, then look the sources up
+#pragma unroll 1
+    for (int i = threadIdx.x; i < c.num_copies; i += kCopyThreads) {
+      const int64_t s = cp_index(c, c.src, i), d = cp_index(c, c.dst, i);
+      if (s < 0 || d < 0 || s >= c.num_units || d >= c.num_units || s == d) continue;
+      uint32_t h = slot(pass ? s : d);
+      while (true) {  // at most half of the slots are taken: it ends
+        const long long old = pass ? table[h] : (long long)atomicCAS((unsigned long long*)&table[h], (unsigned long long)-1ll, (unsigned long long)d);
+        if (old == -1) break;
+        if (old == (pass ? s : d)) {
+          clash = 1;
+          break;
+        }
+        h = (h + 1) & (kHashSlots - 1);
+      }
+    }
+    __syncthreads();
+  }
+  return clash != 0;
+}
+
+// kSplit: one group, whose pairs are spread over blockIdx.y where they do not clash.
+template <bool kSplit>
 __global__ void __launch_bounds__(kCopyThreads, kCopyCtas) copy_units_kernel(const __grid_constant__ CopyParams c) {
   const int64_t cols = c.unit / 16, scols = c.sunit ? c.sunit / c.svec : 0;
   const int64_t parts = (c.num_layers + c.per_thread - 1) / c.per_thread;  // of the layers
   const int64_t at = (int64_t)blockIdx.x * kCopyThreads + threadIdx.x;
-  for (int g = blockIdx.y; g < c.num_groups; g += gridDim.y) {
-    const int64_t first = (int64_t)g * c.num_copies;
+  int begin = 0, end = c.num_copies;
+  if constexpr (kSplit) {
+    const bool whole = pairs_clash(c);
+    if (!whole) {
+      begin = (int)((int64_t)c.num_copies * blockIdx.y / gridDim.y);
+      end = (int)((int64_t)c.num_copies * (blockIdx.y + 1) / gridDim.y);
+    } else if (blockIdx.y > 0) {
+      return;
+    }
+  }
+  for (int g = kSplit ? 0 : blockIdx.y; g < c.num_groups; g += kSplit ? 1 : gridDim.y) {
+    const int64_t first = (int64_t)g * c.num_copies + begin;
     const bool values = at < 2 * parts * cols;
     const int64_t a = values ? at : at - 2 * parts * cols;
     const int64_t n = values ? cols : scols;
@@ -153,16 +201,19 @@ __global__ void __launch_bounds__(kCopyThreads, kCopyCtas) copy_units_kernel(con
       const int64_t part = a / n, col = a - part * n;
       const int l0 = (int)(part >> 1) * c.per_thread, layers = min(c.per_thread, c.num_layers - l0);
       if (values)
-        copy_column<uint4>(c, (part & 1 ? c.base[1] : c.base[0]) + l0 * c.plane_stride + col * 16, c.plane_stride, layers, c.unit, first);
+        copy_column<uint4>(c, (part & 1 ? c.base[1] : c.base[0]) + l0 * c.plane_stride + col * 16, c.plane_stride, layers,
+                           c.unit, first, end - begin);
       else if (c.svec == 16)
-        copy_column<uint4>(c, (part & 1 ? c.sbase[1] : c.sbase[0]) + l0 * c.splane_stride + col * 16, c.splane_stride, layers, c.sunit, first);
+        copy_column<uint4>(c, (part & 1 ? c.sbase[1] : c.sbase[0]) + l0 * c.splane_stride + col * 16, c.splane_stride,
+                           layers, c.sunit, first, end - begin);
       else
-        copy_column<uint32_t>(c, (part & 1 ? c.sbase[1] : c.sbase[0]) + l0 * c.splane_stride + col * 4, c.splane_stride, layers, c.sunit, first);
+        copy_column<uint32_t>(c, (part & 1 ? c.sbase[1] : c.sbase[0]) + l0 * c.splane_stride + col * 4, c.splane_stride,
+                              layers, c.sunit, first, end - begin);
     }
     if (c.invalid_count != nullptr && blockIdx.x == 0) {
       int bad = 0;
-      for (int i = threadIdx.x; i < c.num_copies; i += kCopyThreads) {
-        const int64_t s = cp_index(c, c.src, first + i), d = cp_index(c, c.dst, first + i);
+      for (int i = begin + threadIdx.x; i < end; i += kCopyThreads) {
+        const int64_t s = cp_index(c, c.src, (int64_t)g * c.num_copies + i), d = cp_index(c, c.dst, (int64_t)g * c.num_copies + i);
         bad += s >= 0 && d >= 0 && (s >= c.num_units || d >= c.num_units);
       }
       if (bad) atomicAdd(c.invalid_count, bad);
@@ -220,13 +271,31 @@ int copy_units(const char* fn, void* k_cache, void* v_cache, int32_t cache_dtype
   // against 92 for 253 sequences of up to 7 moves).
   const int64_t unit_cols = c.unit / 16 + (c.sunit ? c.sunit / c.svec : 0);
   const int64_t resident = (int64_t)kNumSMs * kCopyCtas * kCopyThreads;
-  const int64_t waves = (2 * unit_cols * num_layers * (num_groups < 65535 ? num_groups : 65535) + resident - 1) / resident;
+  const int groups = num_groups < 65535 ? num_groups : 65535;
+  const int64_t threads = 2 * unit_cols * num_layers;  // of a group, with a layer each
+  const int64_t waves = (threads * groups + resident - 1) / resident;
   c.per_thread = (int)(waves < 1 ? 1 : waves > 8 ? 8 : waves);
   const int64_t columns = 2 * unit_cols * ((num_layers + c.per_thread - 1) / c.per_thread);
   const int64_t ctas = (columns + kCopyThreads - 1) / kCopyThreads;
   if (ctas > 0x7fffffff) return set_error(MKV_ERR_INVALID_ARGUMENT, "%s: bad sizes", fn);
-  const dim3 grid((unsigned)ctas, (unsigned)(num_groups < 65535 ? num_groups : 65535));
-  copy_units_kernel<<<grid, kCopyThreads, 0, (cudaStream_t)stream>>>(c);
+  // Few columns and many pairs (28 layers of 2 KB pages: 7168 threads, a tenth of what fits): the pairs
+  // are split, in launches of at most kSplitPairs, until the GPU is full or a CTA has kInFlight of them.
+  if (num_groups == 1 && num_copies >= 4 * kInFlight && 2 * threads <= resident) {
+    const int isize = c.i64 ? 8 : 4;
+    for (int64_t i = 0; i < num_copies; i += kSplitPairs) {
+      CopyParams part = c;
+      part.num_copies = (int)(num_copies - i < kSplitPairs ? num_copies - i : kSplitPairs);
+      part.src = (const uint8_t*)src + i * isize;
+      part.dst = (const uint8_t*)dst + i * isize;
+      int64_t splits = resident / threads, most = (part.num_copies + kInFlight - 1) / kInFlight;
+      if (splits > most) splits = most;
+      copy_units_kernel<true><<<dim3((unsigned)ctas, (unsigned)splits), kCopyThreads, 0, (cudaStream_t)stream>>>(part);
+      const int st = cuda_status(cudaGetLastError(), "copy_units launch");
+      if (st != MKV_OK) return st;
+    }
+    return MKV_OK;
+  }
+  copy_units_kernel<false><<<dim3((unsigned)ctas, (unsigned)groups), kCopyThreads, 0, (cudaStream_t)stream>>>(c);
   return cuda_status(cudaGetLastError(), "copy_units launch");
 }
 

@@ -182,6 +182,34 @@ def test_copy_pages_of_any_size_in_any_order(kv, BS, mode):
         assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("pairs", [16, 100, 700, 1024, 1025, 2500])
+@pytest.mark.parametrize("kind", ["apart", "repeated source", "chained", "same destination", "self", "swapped"])
+@pytest.mark.parametrize("mode", ["auto", "int8_per_token_head"])
+def test_many_small_pages(kv, pairs, kind, mode):
+    """Few columns and many pairs: spread over the GPU where no pair touches another's pages, in
+    order where one does, in the first or the last of them."""
+    NB = 2 * pairs + 5
+    c, want = (cache_of(kv, mode, L=2, NB=NB, BS=2, KVH=1, D=32) for _ in range(2))
+    r = random.Random(pairs)
+    perm = r.sample(range(NB), NB)
+    src, dst = perm[:pairs], perm[pairs:2 * pairs]
+    if kind == "repeated source":
+        src = [src[i // 3] for i in range(pairs)]
+    elif kind == "chained":
+        src[-1] = dst[0]
+        src[7] = dst[6]
+    elif kind == "same destination":
+        dst[-1] = dst[1]
+    elif kind == "self":
+        dst[5], dst[9], src[11] = src[5], -1, NB
+    elif kind == "swapped":  # the last one writes what the first one reads
+        dst[-1] = src[0]
+    pages_ref(want, src, dst)
+    kv.copy_kv_pages(c, dev(src), dev(dst))
+    for a, b in zip(planes(c), planes(want)):
+        assert torch.equal(a, b)
+
+
 @pytest.mark.parametrize("mode,dtype,KVH,D", CACHES)
 @pytest.mark.parametrize("G,M", [(1, 1), (1, 5), (5, 9), (11, 30), (1, 0), (0, 3)])
 @pytest.mark.parametrize("index", [torch.int32, torch.int64])
