@@ -20,7 +20,7 @@ namespace {
 // Every type and head_dim (a multiple of 16, at most 256): 16 rows x 32 tokens per step in
 // fp32. A warp owns 4 rows; lane = token for the scores, lane = column for the products.
 constexpr int kGRows = 16, kGKT = 32, kGThreads = 128;
-constexpr int kGCtas = 2 * kNumSMs;
+constexpr int kGCtas = 4 * kNumSMs;  // resident with head_dim up to 128
 
 template <typename CT> __device__ __forceinline__ float elem_f32(const uint8_t* p, int i) {
   return to_f32(reinterpret_cast<const CT*>(p)[i]);
