@@ -723,12 +723,13 @@ class Attention(nn.Module):
             else:
                 store_kvcache(k, v, k_cache, v_cache, context.slot_mapping, self.block_size)
         scale = self.scale / (self.head_dim ** 0.5)
-        if context.tree_mask is not None:  # a step over trees of drafted tokens
+        tree_mask = getattr(context, "tree_mask", None)  # (the reference's own context has none)
+        if tree_mask is not None:  # a step over trees of drafted tokens
             if context.cu_seqlens_q is None or context.context_lens is None or context.block_tables is None:
                 raise ValueError("a tree step requires cu_seqlens_q, context_lens and block_tables")
             o = paged_attention_tree(
                 q, k_cache, v_cache, context.block_tables, context.context_lens, context.cu_seqlens_q,
-                context.tree_mask, scale, self.num_heads, self.num_kv_heads, self.head_dim,
+                tree_mask, scale, self.num_heads, self.num_kv_heads, self.head_dim,
                 self.block_size, self.k_scale, self.v_scale, mode)
             return o.reshape(o.shape[0], self.num_heads * self.head_dim)
         if context.is_prefill:

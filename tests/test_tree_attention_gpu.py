@@ -438,3 +438,14 @@ def test_attention_module_takes_the_tree_branch(attn):
     assert torch.equal(c.k.view(-1, 2, 128)[m.slot_mapping], new_k)
     c.visible = [[{0}, {0, 1}, {0, 2}, {0, 1, 3}, {0, 1, 4}, {0, 1, 4, 5}], [set(range(j + 1)) for j in range(9)]]
     c.check(got.view(15, 8, 128))
+
+
+def test_a_context_without_the_field(attn, monkeypatch):
+    """A runner's own context object, made before trees, still decodes."""
+    import types
+    c = Case(25, [100, 30], [1, 1], 8, 2, 128, 16, BF16, poison=False)
+    layer = attn.Attention(8, 128, 1.0, 2, 16)
+    layer.k_cache, layer.v_cache = c.k, c.v
+    context = types.SimpleNamespace(is_prefill=False, slot_mapping=None, context_lens=c.lens, block_tables=c.bt)
+    monkeypatch.setattr(attn, "get_context", lambda: context)
+    c.check(layer(c.q, None, None).view(2, 8, 128))

@@ -135,6 +135,26 @@ def test_wrappers_refuse(attn):
         kv.move_kv_rows(cache, par.view(1, 3), par.view(1, 3))
 
 
+def test_packed_calls_are_the_calls():
+    """mkv_call_packed passes each word to the parameter it stands for: refusals come out of the
+    same argument, whichever way the call is made."""
+    lib = lib_mod.load()
+    words = dict(q=P, qst=1024, qsh=128, qdt=2, k=P, v=P, cdt=2, ks=0, vs=0, kss=0, vss=0, nb=10, bs=16, bt=P, btt=0,
+                 btst=8, maxb=8, cl=P, clt=1, cu=P, cut=0, mask=P, mst=1, words=1, B=2, T=9, H=8, KVH=2, D=128, scale=0.1,
+                 out=P, ost=1024, osh=128, ws=P, wsb=1 << 40, stream=0)
+    for kw in (dict(H=7), dict(D=100), dict(qdt=3), dict(cdt=4), dict(btt=2), dict(clt=5), dict(cut=9), dict(words=0),
+               dict(bs=0), dict(mask=0), dict(out=0), dict(k=P + 8), dict(wsb=10), dict(ws=P + 4), dict(maxb=1 << 28)):
+        got = lib.mkv_call_packed(lib_mod.CALL_PAGED_TREE_ATTENTION, lib_mod.PACK_TREE_ATTENTION(*{**words, **kw}.values()))
+        message = lib.mkv_last_error()
+        null = {n: v or None for n, v in kw.items() if n in ("mask", "out")}
+        assert got == _tree(lib, **{**kw, **null}) != 0 and message == lib.mkv_last_error()
+    for call, pack, n in ((lib_mod.CALL_TREE_METADATA, lib_mod.PACK_TREE_METADATA, 20),
+                          (lib_mod.CALL_TREE_ACCEPT, lib_mod.PACK_TREE_ACCEPT, 24),
+                          (lib_mod.CALL_COPY_KV_PAGES, lib_mod.PACK_COPY_PAGES, 18),
+                          (lib_mod.CALL_MOVE_KV_ROWS, lib_mod.PACK_MOVE_ROWS, 19)):
+        assert lib.mkv_call_packed(call, pack(*[-1] * n)) != 0
+
+
 def test_the_oracle_itself():
     """The plain implementations on an example worked out by hand."""
     from oracle.tree_oracle import mask_words, tree_accept_ref, tree_metadata_ref

@@ -369,3 +369,67 @@ def test_streams(kv, other):
         got = c.kv.clone()
     s.synchronize()
     assert (got[:, :, 2] == 5).all() and (got[:, :, 3, 0] == 5).all()
+
+
+def test_c_entry_points_and_their_counts(kv):
+    """The C calls themselves (the wrappers make them packed): the same results, and the entries
+    that they skip are counted."""
+    lib_mod = mkv_module("_lib")
+    lib = lib_mod.load()
+    I32, I64 = lib_mod.INDEX_I32, lib_mod.INDEX_I64
+    stream = torch.cuda.current_stream().cuda_stream
+    bad = dev([0], torch.int32)
+    par, cu, pre, bt = dev([-1, 0, 5, -3, 1], torch.int32), dev([0, 3, 5]), dev([4, 9]), dev([[3, 1], [2, 0]], torch.int32)
+    outs = [torch.empty(n, dtype=torch.int64, device=DEV) for n in (5, 2, 5, 5)]
+    st = lib.mkv_tree_metadata(par.data_ptr(), I32, cu.data_ptr(), I64, pre.data_ptr(), I64, bt.data_ptr(), I32, 2, 2, 8, 2,
+                               5, 1, *[o.data_ptr() for o in outs], bad.data_ptr(), stream)
+    lib_mod.check("mkv_tree_metadata", st)
+    m = kv.tree_metadata(par, cu, pre, bt, 8, 3)
+    for a, b in zip(outs, (m.slot_mapping, m.context_lens, m.positions, m.tree_mask.view(-1))):
+        assert torch.equal(a, b)
+    assert bad.tolist() == [3]  # the parents 5, -3 and 1 (of node 1: not a lower one)
+    draft, target = dev([7, 8, 9, 1, 2]), dev([8, 4, 5, 6, 3])
+    par = dev([-1, 0, 0, -1, 0], torch.int32)
+    wide = [torch.empty(2, 4, dtype=torch.int64, device=DEV) for _ in range(3)]
+    nodes, count = torch.empty(2, 4, dtype=torch.int32, device=DEV), dev([0, 0], torch.int32)
+    lens = dev([0, 0])
+    st = lib.mkv_tree_accept(draft.data_ptr(), target.data_ptr(), I64, par.data_ptr(), I32, cu.data_ptr(), I64,
+                             pre.data_ptr(), I64, bt.data_ptr(), I32, 2, 2, 8, 2, 5, 4, count.data_ptr(), nodes.data_ptr(),
+                             wide[0].data_ptr(), lens.data_ptr(), wide[1].data_ptr(), wide[2].data_ptr(), stream)
+    lib_mod.check("mkv_tree_accept", st)
+    a = kv.tree_accept(draft, target, par, cu, pre, bt, 8, 4)
+    for x, y in zip([count, nodes, lens] + wide, (a.num_accepted, a.accepted_nodes, a.context_lens, a.tokens, a.src_slots,
+                                                  a.dst_slots)):
+        assert torch.equal(x, y)
+    for split in (False, True):  # a few pairs, and so many that they are spread over the GPU
+        c, want = (cache_of(kv, "int8_per_token_head", L=2, NB=70, BS=2, KVH=1, D=32) for _ in range(2))
+        src, dst = ([3, -1, 70, 5, 9], [4, 2, 6, 1 << 40, 9]) if not split else \
+            ([3, -1, 70, 5, 9] + list(range(10, 40)), [4, 2, 6, 1 << 40, 8] + list(range(40, 70)))
+        pages_ref(want, src, dst)
+        bad.zero_()
+        s, d = dev(src), dev(dst)
+        k = c.kv.data_ptr()
+        st = lib.mkv_copy_kv_pages(k, k + c.kv.numel() // 2, lib_mod.DTYPE_INT8, 2, 70 * 2 * 32, 70, 2, 1, 32,
+                                   c.k_scale.data_ptr(), c.v_scale.data_ptr(), 140, s.data_ptr(), d.data_ptr(), I64, len(src),
+                                   bad.data_ptr(), stream)
+        lib_mod.check("mkv_copy_kv_pages", st)
+        for x, y in zip(planes(c), planes(want)):
+            assert torch.equal(x, y)
+        assert bad.tolist() == [2]
+    rows_ref(want, [[1, 140, 2]], [[0, 3, 5]])
+    bad.zero_()
+    s, d = dev([[1, 140, 2]]), dev([[0, 3, 5]])
+    st = lib.mkv_move_kv_rows(k, k + c.kv.numel() // 2, lib_mod.DTYPE_INT8, 2, 70 * 2 * 32, 70, 2, 1, 32,
+                              c.k_scale.data_ptr(), c.v_scale.data_ptr(), 140, s.data_ptr(), d.data_ptr(), I64, 1, 3,
+                              bad.data_ptr(), stream)
+    lib_mod.check("mkv_move_kv_rows", st)
+    for x, y in zip(planes(c), planes(want)):
+        assert torch.equal(x, y)
+    assert bad.tolist() == [1]
+
+
+def test_packed_calls_refuse():
+    lib_mod = mkv_module("_lib")
+    lib = lib_mod.load()
+    assert lib.mkv_call_packed(5, b"\0" * 400) == 1 and b"unknown call" in lib.mkv_last_error()
+    assert lib.mkv_call_packed(0, None) == 1 and b"null pointer" in lib.mkv_last_error()
