@@ -67,7 +67,8 @@ struct Layout {
   static constexpr int R0 = V0 + kVS * TILE;
   static constexpr int SC0 = R0 + kRS * 2 * RAW;             // [V stage][K scale, V factor][128]
   static constexpr int QE0 = SC0 + (kTok ? kVS * 2 * kTile * 4 : 0);  // [2][128] exponents of Q's rows
-  static constexpr int BAR0 = QE0 + (kByte ? 2 * kRows : 0);
+  static constexpr int ONE0 = QE0 + (kByte ? 2 * kRows : 0);          // [128] ones: K scales of a masked tile
+  static constexpr int BAR0 = ONE0 + (kTok ? kTile * 4 : 0);
   static constexpr int NBAR = 2 * kKS + 2 * kVS + 2 * kRS + 4 + 2 + 2 + 1 + 2 + 1;
   static constexpr int MISC0 = BAR0 + NBAR * 8;              // tmem base, abort, sick[4], exponents[2], maxima[2][4]
   static constexpr int BYTES = MISC0 + 80;
@@ -157,6 +158,7 @@ paged_tree_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ C
   volatile float* vmax_s = reinterpret_cast<volatile float*>(smem + L::MISC0 + 16 + 4 * kSickSlots);
   int8_t* qexp_s = reinterpret_cast<int8_t*>(smem + L::QE0);
   float* scales_s = reinterpret_cast<float*>(smem + L::SC0);
+  float* ones_s = reinterpret_cast<float*>(smem + L::ONE0);
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
@@ -185,6 +187,7 @@ paged_tree_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ C
     for (int i = 0; i < kSickSlots; ++i) sick_s[i] = 0;
     fence_barrier_init();
   }
+  if (kTok && tid < kTile) ones_s[tid] = 1.0f;
   if (warp == 1) tmem_alloc(tmem_base_s, kTmemCols);
   Walk walk;
   const bool work =
@@ -490,27 +493,36 @@ paged_tree_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ C
           }
         }
         if (warp_live) {
-          // 32 scores: times the tokens' K scales, -inf where the row does not see the token
+          // 32 scores, times the tokens' K scales
+          const float* kscale = ksp;
           auto scores = [&](int h, float (&v)[32]) {
             tmem_ld32(sa + 32 * h, v);
             if constexpr (kTok) {
 #pragma unroll
               for (int e = 0; e < 32; e += 4) {
-                const float4 k4 = *reinterpret_cast<const float4*>(ksp + 32 * h + e);
+                const float4 k4 = *reinterpret_cast<const float4*>(kscale + 32 * h + e);
                 v[e] *= k4.x;
                 v[e + 1] *= k4.y;
                 v[e + 2] *= k4.z;
                 v[e + 3] *= k4.w;
               }
             }
-            if (special) {
+          };
+          if (special) {  // the mask is put into S (and the K scales with it), so that the loops below have none
+#pragma unroll 1
+            for (int h = 0; h < 4; ++h) {
+              float v[32];
+              scores(h, v);
               const uint32_t vis = visible(h);
               seen |= vis != 0u;
+              uint32_t w[32];
 #pragma unroll
-              for (int e = 0; e < 32; ++e)
-                if (!((vis >> e) & 1u)) v[e] = -INFINITY;
+              for (int e = 0; e < 32; ++e) w[e] = (vis >> e) & 1u ? __float_as_uint(v[e]) : 0xff800000u;
+              tmem_st32(sa + 32 * h, w);
             }
-          };
+            tmem_wait_st();
+            if constexpr (kTok) kscale = ones_s;
+          }
           // the tile's maximum, then P, 32 columns at a time (S is read twice: that costs less
           // than the registers to hold it, whose spills miss an L1 that shared memory has
           // taken; and short loops keep the roles' code in the instruction cache)
