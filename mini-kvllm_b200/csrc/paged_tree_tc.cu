@@ -429,9 +429,7 @@ paged_tree_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ C
       sc0 *= __ldg(p.k_scale);
       vs0 = __ldg(p.v_scale);
     }
-    // positive (the rows of Q take a negative sign) and not 0, so that a masked -inf stays one
-    sc0 = fabsf(sc0);
-    if (sc0 < 1e-30f) sc0 = 1e-30f;
+    sc0 = fabsf(sc0);  // the rows of Q take a negative sign
 #pragma unroll 1
     while (ok && next<kRows, kTile>(p, walk, u)) {
       const int tiles = u.k1 - u.k0;
@@ -448,6 +446,7 @@ paged_tree_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ C
         if (!(ok = wait(&qfull[unit & 1], unit >> 1))) break;
         sc *= pow2f(-(int)qexp_s[(unit & 1) * kRows + rt]);
       }
+      if (sc < 1e-37f) sc = 1e-37f;  // not 0, so that a masked -inf stays one
       float m = -INFINITY, l = 0.0f;  // reference (exp2 domain) and sum of this stream
       int vexp = 0;                   // O holds values times 2^-vexp (kTok)
       bool seen = false;
@@ -481,8 +480,10 @@ paged_tree_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ C
         const float* ksp = scales_s + st * 2 * kTile;
         float alpha = 1.0f;
         bool rescale = false;
-        if constexpr (kTok) {  // the converters have written the tile's scales
+        if (kByte && (kTok || special)) {  // the converters have written the tile's scales and flags
           if (!(ok = wait(&vfull[st], vph))) break;
+        }
+        if constexpr (kTok) {
           const int e = vexp_s[st];
           if (e != vexp) {
             if (ns != 0) {
@@ -705,6 +706,7 @@ paged_tree_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ C
     };
     auto row_of = [&](int t, Entry e) -> int64_t {
       const int64_t page = t < u.s.len ? page_of(p, e) : -1;
+      if constexpr (!kTok) return page;  // (whether there is one is all that matters)
       return page < 0 ? -1 : (page * p.block_size + (t & (p.block_size - 1))) * p.num_kv_heads + u.kvh;
     };
     auto convert = [&](const uint8_t* src, uint8_t* dst, bool valid) {

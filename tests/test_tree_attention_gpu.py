@@ -326,6 +326,14 @@ def test_many_sequences(attn):
     c.check(c.run(attn))
 
 
+@pytest.mark.parametrize("mode", ["auto", "fp8_per_tensor"])
+def test_more_sequences_than_any_block_has_threads(attn, mode):
+    r = random.Random(26)
+    c = Case(26, [r.choice([0, 1, 17, 40]) for _ in range(1100)], [r.choice([0, 1, 2, 5]) for _ in range(1100)], 4, 2, 64,
+             16, BF16, mode)
+    c.check(c.run(attn))
+
+
 def test_pages_past_32_bits(attn):
     """A cache of 2^31 + elements: byte and element offsets beyond 32 bits."""
     NB, BS, KVH, D = 70000, 256, 1, 128  # 2.3e9 elements
@@ -352,6 +360,9 @@ def test_negative_and_zero_scales(attn):
             c = Case(22, [200, 3], [9, 20], 8, 2, 128, 16, dtype, mode)
             c.scale = scale
             c.check(c.run(attn))
+            if dtype == BF16:  # tiny queries too: their f16 form has a power of two of its own
+                c.q = (c.q.float() * 2.0 ** -70).to(BF16)
+                c.check(c.run(attn))
 
 
 @pytest.mark.parametrize("size", [1e-6, 1e4])
