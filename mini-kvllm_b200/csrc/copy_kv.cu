@@ -14,9 +14,10 @@
 //
 // Bound: memory, 2 x unit bytes a copy. The columns of a whole cache (28 layers of 32 KB
 // pages: 114688) keep 14 MB in flight, enough to cover the latency of HBM, and their threads
-// fit the GPU at once (233 pairs: 140 us, 6.1 TB/s, 0.93 of the copy rate; three pairs 3.6 us). Where the columns are few and the pairs many (small pages of one kv
-// head), the pairs are split over CTAs as well, if none of them writes what another one reads or
-// writes: every CTA finds that out for itself, with a hash table of the destinations.
+// fit the GPU at once (233 pairs: 140 us, 6.1 TB/s, 0.93 of the copy rate; three pairs 3.6 us).
+// Where the columns are few and the pairs many (small pages of one kv head), the pairs are split
+// over CTAs as well, if none of them writes what another one reads or writes: every CTA finds
+// that out for itself, with a hash table of the destinations.
 // A group of row copies is one sequence's, groups side by side; there a
 // thread's layers share the reading and checking of the indices.
 #include "mkv_common.cuh"
@@ -162,7 +163,9 @@ __device__ bool pairs_clash(const CopyParams& c) {
       if (s < 0 || d < 0 || s >= c.num_units || d >= c.num_units || s == d) continue;
       uint32_t h = slot(pass ? s : d);
       while (true) {  // at most half of the slots are taken: it ends
-        const long long old = pass ? table[h] : (long long)atomicCAS((unsigned long long*)&table[h], (unsigned long long)-1ll, (unsigned long long)d);
+        const long long old = pass ? table[h]
+                                   : (long long)atomicCAS((unsigned long long*)&table[h], (unsigned long long)-1ll,
+                                                          (unsigned long long)d);
         if (old == -1) break;
         if (old == (pass ? s : d)) {
           clash = 1;
@@ -213,7 +216,8 @@ __global__ void __launch_bounds__(kCopyThreads, kCopyCtas) copy_units_kernel(con
     if (c.invalid_count != nullptr && blockIdx.x == 0) {
       int bad = 0;
       for (int i = begin + threadIdx.x; i < end; i += kCopyThreads) {
-        const int64_t s = cp_index(c, c.src, (int64_t)g * c.num_copies + i), d = cp_index(c, c.dst, (int64_t)g * c.num_copies + i);
+        const int64_t at = (int64_t)g * c.num_copies + i;
+        const int64_t s = cp_index(c, c.src, at), d = cp_index(c, c.dst, at);
         bad += s >= 0 && d >= 0 && (s >= c.num_units || d >= c.num_units);
       }
       if (bad) atomicAdd(c.invalid_count, bad);

@@ -185,7 +185,8 @@ __global__ void __launch_bounds__(kGThreads) paged_tree_generic_kernel(const __g
 #pragma unroll
         for (int i = 0; i < 8; ++i)
           if (lane + 32 * i < D) a[lane + 32 * i] = acc[r][i];
-        if (lane == 0)           p.part_ml[(int64_t)slot * kGRows + row] = make_float2(m[r], l[r] == 0.0f && any[r] ? kSeenInf : l[r]);
+        if (lane == 0)
+          p.part_ml[(int64_t)slot * kGRows + row] = make_float2(m[r], l[r] == 0.0f && any[r] ? kSeenInf : l[r]);
       }
     }
   }
@@ -351,7 +352,8 @@ extern "C" int mkv_paged_tree_attention(
     return set_error(MKV_ERR_INVALID_ARGUMENT, "%s: scales given for an unquantised cache", fn);
   if (byte && (tensor_scales == row_scales || (tensor_scales && (!k_scale || !v_scale)) ||
                (row_scales && (!k_scales || !v_scales))))
-    return set_error(MKV_ERR_INVALID_ARGUMENT, "%s: an 8-bit cache needs k_scale and v_scale, or k_scales and v_scales", fn);
+    return set_error(MKV_ERR_INVALID_ARGUMENT,
+                     "%s: an 8-bit cache needs k_scale and v_scale, or k_scales and v_scales", fn);
   if (cache_dtype == MKV_DTYPE_INT8 && !row_scales)
     return set_error(MKV_ERR_INVALID_ARGUMENT, "%s: an INT8 cache needs k_scales and v_scales", fn);
   if (num_seqs == 0 || total_q == 0) return MKV_OK;

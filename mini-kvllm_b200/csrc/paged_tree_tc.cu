@@ -110,7 +110,8 @@ __device__ __noinline__ bool clear_sick(uint8_t* row, int bytes) {
     bool here = false;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const uint32_t keep = ((w[e] & kExp) == kExp ? 0u : 0x0000ffffu) | ((w[e] >> 16 & kExp) == kExp ? 0u : 0xffff0000u);
+      const uint32_t keep = ((w[e] & kExp) == kExp ? 0u : 0x0000ffffu) |
+                            ((w[e] >> 16 & kExp) == kExp ? 0u : 0xffff0000u);
       here |= keep != 0xffffffffu;
       w[e] &= keep;
     }
@@ -252,7 +253,8 @@ paged_tree_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ C
       for (int i = 0; i <= tiles && ok; ++i) {
         const int64_t page_k = i < tiles ? seg_page(u, u.k0 + i, next_e) : -1;
         if (i + 1 < tiles) next_e = seg_entry(u, u.k0 + i + 1);
-        if (i + 8 < tiles && seg_in(u, u.k0 + i + 8)) prefetch_entry(p, u.b, ((u.k0 + i + 8) * kTile + lane * seg_rows) >> bs_log2);
+        if (i + 8 < tiles && seg_in(u, u.k0 + i + 8))
+          prefetch_entry(p, u.b, ((u.k0 + i + 8) * kTile + lane * seg_rows) >> bs_log2);
         if constexpr (kByte) {
           if (i == tiles) break;
           const uint32_t st = nk % kRS;

@@ -234,24 +234,6 @@ __device__ __forceinline__ void tmem_st16u(uint32_t taddr, const uint32_t (&w)[1
       : "memory");
 }
 
-// 4 consecutive 32-bit columns of this thread's TMEM lane, each with its wait.
-__device__ __forceinline__ void tmem_st4(uint32_t taddr, float a, float b, float c, float d) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1,%2,%3,%4};\n\t"
-               "tcgen05.wait::st.sync.aligned;" ::"r"(taddr), "r"(__float_as_uint(a)),
-               "r"(__float_as_uint(b)), "r"(__float_as_uint(c)), "r"(__float_as_uint(d))
-               : "memory");
-}
-__device__ __forceinline__ void tmem_ld4(uint32_t taddr, float (&v)[4]) {
-  uint32_t r[4];
-  asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0,%1,%2,%3}, [%4];\n\t"
-               "tcgen05.wait::ld.sync.aligned;"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(taddr)
-               : "memory");
-#pragma unroll
-  for (int i = 0; i < 4; ++i) v[i] = __uint_as_float(r[i]);
-}
-
 // One lane of a converged warp, chosen by the hardware: the branch on it is known to be
 // uniform, so the operands of what it guards can live in uniform registers.
 __device__ __forceinline__ bool elect_one() {

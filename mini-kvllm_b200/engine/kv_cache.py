@@ -328,7 +328,8 @@ def _cache_args(fn: str, cache: KVCache):
     if cache.kv_cache_dtype in PER_TOKEN_HEAD:
         for t in (cache.k_scale, cache.v_scale):
             if t is None or t.dtype != torch.float32 or t.shape != (L, NB, BS, KVH) or not t.is_contiguous():
-                raise ValueError(f"{fn}: {cache.kv_cache_dtype} needs contiguous float32 scales ({L}, {NB}, {BS}, {KVH})")
+                raise ValueError(f"{fn}: {cache.kv_cache_dtype} needs contiguous float32 scales "
+                                 f"({L}, {NB}, {BS}, {KVH})")
         ks, vs, stride = cache.k_scale.data_ptr(), cache.v_scale.data_ptr(), NB * BS * KVH
     k = kv.data_ptr()
     v = k + kv.numel() // 2 * kv.element_size()
