@@ -14,7 +14,7 @@
 //
 // Bound: memory, 2 x unit bytes a copy. The columns of a whole cache (28 layers of 32 KB
 // pages: 114688) keep 14 MB in flight, enough to cover the latency of HBM, and their threads
-// fit the GPU at once (233 pairs: 140 us, 6.1 TB/s, 0.93 of the copy rate; three pairs 3.6 us).
+// fit the GPU at once (233 pairs: 140 us, 6.1 TB/s, 0.94 of the copy rate; three pairs 3.4 us).
 // Where the columns are few and the pairs many (small pages of one kv head), the pairs are split
 // over CTAs as well, if none of them writes what another one reads or writes: every CTA finds
 // that out for itself, with a hash table of the destinations.

@@ -18,11 +18,11 @@
 // tile, 1.5 us of an SM's share of HBM; its two products 0.55 us).
 //
 // Measured (B200, device time of the call with its combine): bf16, 48 sequences of 1-8k tokens, 8-32
-// nodes, 32/8 heads 174 us, 5.35 TB/s (0.82 of the copy rate), DRAM reads 0.94 GB = K and V once;
-// e4m3, 12 x 32k, 32 nodes 250 us, 825 TFLOP/s, tensor pipe 39 % and exponentials 39 % busy: a tile
+// nodes, 32/8 heads 172 us, 5.42 TB/s (0.83 of the copy rate), DRAM reads 0.94 GB = K and V once;
+// e4m3, 12 x 32k, 32 nodes 246 us, 838 TFLOP/s, tensor pipe 39 % and exponentials 39 % busy: a tile
 // takes 2500 clocks, of them 1050 each for the exponentials, the products and (four warps) the
 // conversions, in a chain that two streams overlap by half; int8 with row scales, 19 x 1-5k over
-// 16-token pages 80 us. Two streams, not one shared accumulator or half a tile per warpgroup: both
+// 16-token pages 77 us. Two streams, not one shared accumulator or half a tile per warpgroup: both
 // measured slower (250-270 us against 319 and 391 for e4m3).
 //
 // What a row must not see: scores of hidden tokens are replaced by -inf before the maximum.

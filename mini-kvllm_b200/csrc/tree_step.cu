@@ -14,8 +14,8 @@
 // Both are bound by launch and load latency (a batch of 256 trees of 64 nodes holds half a
 // megabyte), so each is one launch, with a chain of dependent loads that does not grow
 // with the number of nodes: a tree is read once, into shared memory or registers, and
-// walked there. Measured (B200, graph replays): metadata of 1 / 256 trees 2.8 / 3.4 us,
-// acceptance 3.2 / 5.3 us, about what an empty launch takes.
+// walked there. Measured (B200, graph replays): metadata of 1 / 256 trees 2.6 / 3.3 us,
+// acceptance 2.9 / 5.1 us, about what an empty launch takes.
 #include "mkv_common.cuh"
 
 namespace mkv {
