@@ -14,8 +14,8 @@
 // Both are bound by launch and load latency (a batch of 256 trees of 64 nodes holds half a
 // megabyte), so each is one launch, with a chain of dependent loads that does not grow
 // with the number of nodes: a tree is read once, into shared memory or registers, and
-// walked there. Measured (B200, graph replays): metadata of 1 / 256 trees 2.6 / 3.3 us,
-// acceptance 2.9 / 5.1 us, about what an empty launch takes.
+// walked there. Measured (B200, graph replays): metadata of 1 / 256 trees 2.8 / 3.4 us,
+// acceptance 3.1 / 5.1 us, about what an empty launch takes.
 #include "mkv_common.cuh"
 
 namespace mkv {
@@ -50,10 +50,10 @@ __device__ __forceinline__ int64_t ts_prefix(const TreeParams& p, int b) {
   return max(ts_index(p.prefix, p.prefix_i64, b), (int64_t)0);
 }
 
-// Cache slot of position pos of sequence b, -1 where it has no page.
-__device__ __forceinline__ int64_t ts_slot(const TreeParams& p, int b, int64_t pos) {
-  const int64_t blk = pos / p.block_size;
-  if (blk >= p.max_blocks) return -1;
+// Cache slot of token `j` behind the prefix of sequence b, -1 where it has no page.
+__device__ __forceinline__ int64_t ts_slot(const TreeParams& p, int b, int64_t prefix, int64_t j) {
+  if (prefix >= (int64_t)p.max_blocks * p.block_size - j) return -1;  // (the sum may pass 64 bits)
+  const int64_t pos = prefix + j, blk = pos / p.block_size;
   const int64_t page = ts_index(p.bt, p.bt_i64, b * p.bt_stride + blk);
   return page < 0 ? -1 : page * p.block_size + (pos - blk * p.block_size);
 }
@@ -106,7 +106,7 @@ tree_metadata_kernel(const TreeParams p, int words, int64_t* slots, int64_t* len
       acc |= 1ull << (a & 63);
     }
     for (; w >= 0; acc = 0) row[w--] = acc;
-    slots[q0 + j] = ts_slot(p, b, prefix + j);
+    slots[q0 + j] = ts_slot(p, b, prefix, j);
     positions[q0 + j] = prefix + depth;
   }
   for (int64_t j = n + tid; j < n64; j += kMetaThreads) {  // past the mask's width: not cached, sees nothing
@@ -157,8 +157,8 @@ tree_accept_kernel(const TreeParams p, const void* draft, const void* target, in
     row_n[e] = (int32_t)my_node;
     row_t[e] = my_tok;
     const bool moved = my_node >= 0 && my_node != e;
-    src[(int64_t)b * max_path + e] = moved ? ts_slot(p, b, prefix + my_node) : -1;
-    dst[(int64_t)b * max_path + e] = moved ? ts_slot(p, b, prefix + e) : -1;
+    src[(int64_t)b * max_path + e] = moved ? ts_slot(p, b, prefix, my_node) : -1;
+    dst[(int64_t)b * max_path + e] = moved ? ts_slot(p, b, prefix, e) : -1;
     my_node = my_tok = -1;
   };
   for (k = 0; k < max_path; ++k) {
@@ -237,8 +237,9 @@ extern "C" int mkv_tree_metadata(const void* parents, int32_t parents_index_type
   if (st != MKV_OK) return st;
   if (mask_words < 1 || mask_words > kMaxWords)
     return set_error(MKV_ERR_UNSUPPORTED, "%s: mask_words must be 1 to %d (got %d)", fn, kMaxWords, mask_words);
-  if (num_seqs == 0) return MKV_OK;
-  if (!context_lens || (total_q > 0 && (!slot_mapping || !positions || !tree_mask)))
+  if (num_seqs == 0 && total_q == 0) return MKV_OK;
+  if (!cu_seqlens_q) return set_error(MKV_ERR_INVALID_ARGUMENT, "%s: null pointer argument", fn);
+  if ((num_seqs > 0 && !context_lens) || (total_q > 0 && (!slot_mapping || !positions || !tree_mask)))
     return set_error(MKV_ERR_INVALID_ARGUMENT, "%s: null output pointer", fn);
   TreeParams p{parents, cu_seqlens_q, prefix_lens, block_tables, block_table_stride_seq,
                parents_index_type == MKV_INDEX_I64, cu_seqlens_index_type == MKV_INDEX_I64,

@@ -67,7 +67,8 @@ def test_nothing_to_do():
 @pytest.mark.parametrize("kw,status,msg", [
     (dict(pt=7), 1, b"index types"), (dict(words=0), 2, b"mask_words"), (dict(words=17), 2, b"mask_words"),
     (dict(bs=0), 1, b"bad sizes"), (dict(B=-2), 1, b"bad sizes"), (dict(cu=None), 1, b"null pointer"),
-    (dict(slots=None), 1, b"null output"), (dict(bt=None), 1, b"null pointer")])
+    (dict(slots=None), 1, b"null output"), (dict(bt=None), 1, b"null pointer"),
+    (dict(B=0, cu=None), 1, b"null pointer"), (dict(B=0, slots=None), 1, b"null output")])
 def test_metadata_refusals(kw, status, msg):
     a = dict(par=P, pt=0, cu=P, ct=0, pre=P, prt=1, bt=P, btt=0, bts=4, maxb=4, bs=16, B=2, T=5, words=1, slots=P, lens=P,
              pos=P, mask=P, bad=None, stream=None)

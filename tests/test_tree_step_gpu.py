@@ -83,6 +83,25 @@ def test_metadata_of_padding_bad_parents_and_missing_pages(kv):
     assert torch.equal(m.tree_mask.cpu(), want)
 
 
+@pytest.mark.parametrize("cu", [0, 3])
+def test_metadata_of_padding_alone(kv, cu):
+    """A step that is all padding (no sequence): slot -1 everywhere, so the append writes nothing."""
+    m = kv.tree_metadata(dev([-1, 0, 1, 2, 0], torch.int32), dev([cu]), dev([]),
+                         torch.zeros(0, 4, dtype=torch.int32, device=DEV), 16, 70)
+    assert m.slot_mapping.tolist() == [-1] * 5 and m.positions.tolist() == [0] * 5
+    assert m.context_lens.numel() == 0 and not m.tree_mask.any() and m.tree_mask.shape == (5, 2)
+
+
+def test_prefix_past_64_bits_has_no_slots(kv):
+    top = 2**63 - 1
+    tables = dev([[0, 1], [1, 0]], torch.int32)
+    m = kv.tree_metadata(dev([-1, 0, 0, -1], torch.int32), dev([0, 3, 4]), dev([top, 5]), tables, 16, 8)
+    assert m.slot_mapping.tolist() == [-1] * 3 + [21]
+    a = kv.tree_accept(dev([7, 8, 9, 7]), dev([9, 0, 0, 0]), dev([-1, 0, 0, -1], torch.int32), dev([0, 3, 4]), dev([top, 5]),
+                       tables, 16, 3)
+    assert a.accepted_nodes[0].tolist() == [0, 2, -1] and (a.src_slots == -1).all() and (a.dst_slots == -1).all()
+
+
 @pytest.mark.parametrize("nodes", [[1], [8], [0, 5, 0, 64, 129, 300], [40] * 70])
 @pytest.mark.parametrize("max_path", [1, 4, 9, 40])
 @pytest.mark.parametrize("tok", [torch.int32, torch.int64])
