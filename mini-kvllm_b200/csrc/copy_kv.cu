@@ -86,7 +86,8 @@ __device__ __forceinline__ void cp_store(uint8_t* p, bool on, uint32_t v) {
 
 // All copies of one column of a group in `layers` layers, `stride` bytes apart: p points at its
 // bytes in unit 0 of the first, T is its type. A negative entry is no copy; one past the cache
-// is skipped.
+// is skipped. A unit's copy onto itself is left out: done as a load and a store it would put old
+// bytes over those that another CTA, with another part of the pairs, has copied there.
 template <typename T>
 __device__ __forceinline__ void copy_column(const CopyParams& c, uint8_t* p, int64_t stride, int layers,
                                             int64_t unit, int64_t first, int count) {
@@ -101,7 +102,7 @@ __device__ __forceinline__ void copy_column(const CopyParams& c, uint8_t* p, int
         s[u] = cp_index(c, c.src, first + i0 + u);
         d[u] = cp_index(c, c.dst, first + i0 + u);
       }
-      if (s[u] < 0 || d[u] < 0 || s[u] >= c.num_units || d[u] >= c.num_units) s[u] = d[u] = -1;
+      if (s[u] < 0 || d[u] < 0 || s[u] >= c.num_units || d[u] >= c.num_units || s[u] == d[u]) s[u] = d[u] = -1;
       any |= s[u] >= 0;
 #pragma unroll
       for (int w = 0; w < u; ++w) chained |= s[u] >= 0 && s[u] == d[w];
@@ -145,8 +146,8 @@ __device__ __forceinline__ void copy_column(const CopyParams& c, uint8_t* p, int
   }
 }
 
-// Whether some pair of c writes a unit that another one reads or writes. Block-collective; the
-// same answer in every block.
+// Whether some pair of c writes a unit that another one reads or writes (copies of a unit onto
+// itself read and write nothing). Block-collective; the same answer in every block.
 __device__ bool pairs_clash(const CopyParams& c) {
   __shared__ long long table[kHashSlots];
   __shared__ int clash;

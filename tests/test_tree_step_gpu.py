@@ -229,6 +229,36 @@ def test_many_small_pages(kv, pairs, kind, mode):
         assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("pairs", [16, 100, 1025])
+@pytest.mark.parametrize("rows", [False, True])
+@pytest.mark.parametrize("mode", ["auto", "int8_per_token_head"])
+def test_copies_onto_themselves_beside_copies_there(kv, pairs, rows, mode):
+    """Padding a plan with copies of a unit onto itself changes nothing, although another pair, in
+    the first or the last part of the plan, fills that unit: whatever the order of the two, the
+    filled unit stays filled."""
+    n = 2 * pairs + 5
+    BS = 1 if rows else 2
+    for first, last in ((0, pairs - 1), (pairs - 1, 0), (1, pairs // 2), (pairs // 2, 1)):
+        c, want = (cache_of(kv, mode, L=2, NB=n, BS=BS, KVH=1, D=32, seed=first) for _ in range(2))
+        r = random.Random(pairs + first)
+        perm = r.sample(range(n), n)
+        src, dst = perm[:pairs], perm[pairs:2 * pairs]
+        src[first] = dst[first] = dst[last]  # onto itself, a destination of the pair `last`
+        if pairs > 16:
+            src[7] = dst[7] = dst[-2]
+        if rows:
+            rows_ref(want, [src], [dst])
+        else:
+            pages_ref(want, src, dst)
+        for _ in range(5):  # (again: the sources are no destinations, so the result is the same)
+            if rows:
+                kv.move_kv_rows(c, dev([src]), dev([dst]))
+            else:
+                kv.copy_kv_pages(c, dev(src), dev(dst))
+            for a, b in zip(planes(c), planes(want)):
+                assert torch.equal(a, b)
+
+
 @pytest.mark.parametrize("mode,dtype,KVH,D", CACHES)
 @pytest.mark.parametrize("G,M", [(1, 1), (1, 5), (5, 9), (11, 30), (1, 0), (0, 3)])
 @pytest.mark.parametrize("index", [torch.int32, torch.int64])
