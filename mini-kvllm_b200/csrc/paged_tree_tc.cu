@@ -69,9 +69,9 @@ struct Layout {
   static constexpr int QE0 = SC0 + (kTok ? kVS * 2 * kTile * 4 : 0);  // [2][128] exponents of Q's rows
   static constexpr int ONE0 = QE0 + (kByte ? 2 * kRows : 0);          // [128] ones: K scales of a masked tile
   static constexpr int BAR0 = ONE0 + (kTok ? kTile * 4 : 0);
-  static constexpr int NBAR = 2 * kKS + 2 * kVS + 2 * kRS + 4 + 2 + 2 + 1 + 2 + 1;
+  static constexpr int NBAR = 2 * kKS + 2 * kVS + 2 * kRS + 4 + 2 + 2 + 1 + 2 + 1 + 1;
   static constexpr int MISC0 = BAR0 + NBAR * 8;              // tmem base, abort, sick[4], exponents[2], maxima[2][4]
-  static constexpr int BYTES = MISC0 + 80;
+  static constexpr int BYTES = MISC0 + 64;
   static_assert(BYTES <= 232448, "shared memory per CTA");
   static_assert(kBeginWords(kThreads) * 8 <= TILE, "the schedule's scratch lies in the first K stage");
 };
@@ -152,6 +152,7 @@ paged_tree_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ C
   uint64_t* ofull = pfull + 2;
   uint64_t* xbar = ofull + 1;
   uint64_t* drain = xbar + 2;
+  uint64_t* cbar = drain + 1;
   uint32_t* tmem_base_s = reinterpret_cast<uint32_t*>(smem + L::MISC0);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::MISC0 + 4);
   volatile int* sick_s = reinterpret_cast<volatile int*>(smem + L::MISC0 + 8);
@@ -184,6 +185,7 @@ paged_tree_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ C
     }
     mbar_init(ofull, 1);
     mbar_init(drain, 1);
+    mbar_init(cbar, 4);
     *abort_flag = 0;
     for (int i = 0; i < kSickSlots; ++i) sick_s[i] = 0;
     fence_barrier_init();
@@ -778,8 +780,12 @@ paged_tree_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ C
           }
           const float wm = warp_max(isfinite(vs) ? fabsf(vs) : 0.0f);
           volatile float* mx = vmax_s + 4 * (k & 1);  // two sets: the other one may still be read
-          if (lane == 0) mx[warp - 12] = wm;
-          asm volatile("bar.sync 1, 128;" ::: "memory");
+          if (lane == 0) {
+            mx[warp - 12] = wm;
+            mbar_arrive(cbar);
+          }
+          __syncwarp();
+          if (!(ok = wait(cbar, k))) break;  // (bounded as every wait: another converter may have given up)
           const float tm = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
           if (tm > 0.0f) {
             const int e = min(max((int)(__float_as_uint(tm) >> 23) - 127, -100), 100);

@@ -165,3 +165,20 @@ def test_the_oracle_itself():
     assert mask_words(visible, 1).tolist() == [[1], [3], [5], [13], [21]]
     got = tree_accept_ref([9, 5, 6, 8, 8], [6, 1, 8, 2, 3], parents, cu, [14], tables, 16, 4)
     assert got == ([3], [[0, 2, 3, -1]], [[6, 8, 2, -1]], [17], [[-1, 64, 65, -1]], [[-1, 127, 64, -1]])
+
+
+def test_the_roles_of_a_kernel_meet_at_bounded_barriers_only():
+    """A warp that gives up a wait leaves its loop. What the others wait for then has to have a
+    limit: no barrier over a part of the threads (bar / barrier with a number of its own), and no
+    loop on an mbarrier but the one in mbar_wait, which counts the clocks."""
+    import pathlib
+    import re
+    csrc = pathlib.Path(lib_mod.PKG_DIR) / "csrc"
+    files = sorted(csrc.glob("*.cu*"))
+    assert files
+    for f in files:
+        code = re.sub(r"//[^\n]*", "", f.read_text())
+        assert not re.search(r"\b(bar|barrier)(\.cta)?\.(sync|red|arrive)", code), f.name
+        assert not re.search(r"__barrier_sync|named_barrier|cuda::barrier", code), f.name
+        waits = [m.start() for m in re.finditer(r"mbarrier\.try_wait|mbarrier\.test_wait", code)]
+        assert len(waits) == (1 if f.name == "sm100.cuh" else 0), f.name
