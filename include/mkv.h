@@ -518,7 +518,8 @@ MKV_API int mkv_tree_metadata(const void* parents, int32_t parents_index_type, c
  *     out[row, h] = softmax_t(scale * query[row, h] . K[t, kvh(h)]) V[t, kvh(h)]
  * over what it sees, in fp32, kvh(h) = h / (num_heads / num_kv_heads). A row that sees
  * nothing gives zeros. Tokens on a page entry that is -1 or out of range, or past
- * max_num_blocks * block_size, are skipped. Rows of no sequence are left as they are.
+ * max_num_blocks * block_size, are skipped. Rows of no sequence are left as they are, and set to
+ * 0 by the _zeroed variant (every row is, where num_seqs is 0).
  * K/V that a row does not see may hold anything (infinities and NaN included).
  * Caches: the query's dtype (bf16, f16, f32), FP8_E4M3 with k_scale / v_scale (one float
  * each) or with k_scales / v_scales per (page, row, kv head), INT8 with k_scales /
@@ -531,6 +532,17 @@ MKV_API size_t mkv_paged_tree_workspace_bytes(int32_t num_seqs, int64_t total_q,
                                               int32_t num_kv_heads, int32_t head_dim, int32_t q_dtype,
                                               int32_t cache_dtype);
 MKV_API int mkv_paged_tree_attention(
+    const void* query, int64_t q_stride_token, int64_t q_stride_head, int32_t q_dtype,
+    const void* k_cache, const void* v_cache, int32_t cache_dtype, const float* k_scale,
+    const float* v_scale, const float* k_scales, const float* v_scales, int64_t num_blocks,
+    int32_t block_size, const void* block_tables, int32_t block_table_index_type,
+    int64_t block_table_stride_seq, int32_t max_num_blocks, const void* context_lens,
+    int32_t context_lens_index_type, const void* cu_seqlens_q, int32_t cu_seqlens_index_type,
+    const uint64_t* tree_mask, int64_t mask_stride_token, int32_t mask_words, int32_t num_seqs,
+    int64_t total_q, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim, float scale,
+    void* out, int64_t out_stride_token, int64_t out_stride_head, void* workspace,
+    size_t workspace_bytes, void* stream);
+MKV_API int mkv_paged_tree_attention_zeroed(
     const void* query, int64_t q_stride_token, int64_t q_stride_head, int32_t q_dtype,
     const void* k_cache, const void* v_cache, int32_t cache_dtype, const float* k_scale,
     const float* v_scale, const float* k_scales, const float* v_scales, int64_t num_blocks,
@@ -595,7 +607,7 @@ MKV_API int mkv_move_kv_rows(void* k_cache, void* v_cache, int32_t cache_dtype, 
                              int32_t* invalid_count, void* stream);
 
 /*
- * The five calls above with their arguments, in the same order, as an array of 64-bit words:
+ * The calls above with their arguments, in the same order, as an array of 64-bit words:
  * pointers and integers as they are, a float as the bits of a double. For bindings in which
  * every argument of a foreign call has a cost of its own (ctypes: a quarter of a microsecond
  * each, more than these kernels' launch in sum).
@@ -605,6 +617,7 @@ MKV_API int mkv_move_kv_rows(void* k_cache, void* v_cache, int32_t cache_dtype, 
 #define MKV_CALL_TREE_ACCEPT 2
 #define MKV_CALL_COPY_KV_PAGES 3
 #define MKV_CALL_MOVE_KV_ROWS 4
+#define MKV_CALL_ZEROED 0x100 /* added to MKV_CALL_PAGED_TREE_ATTENTION: its _zeroed variant */
 MKV_API int mkv_call_packed(int32_t call, const int64_t* args);
 
 #ifdef __cplusplus

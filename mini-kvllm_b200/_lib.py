@@ -25,7 +25,7 @@ AR_MAX_RANKS, AR_MAX_BLOCKS, IPC_HANDLE_BYTES = 8, 128, 64
 AR_FLAG_BYTES = AR_MAX_BLOCKS * AR_MAX_RANKS * 4
 
 CALL_PAGED_TREE_ATTENTION, CALL_TREE_METADATA, CALL_TREE_ACCEPT = 0, 1, 2
-CALL_COPY_KV_PAGES, CALL_MOVE_KV_ROWS = 3, 4
+CALL_COPY_KV_PAGES, CALL_MOVE_KV_ROWS, CALL_ZEROED = 3, 4, 0x100
 
 # Every symbol include/mkv.h declares, with (restype, argtypes).
 _p, _i32, _i64, _f32, _sz = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64, ctypes.c_float, ctypes.c_size_t
@@ -77,6 +77,9 @@ SIGNATURES: dict[str, tuple] = {
         _p, _i32, _p, _i32, _p, _i32, _p, _i32, _i64, _i32, _i32, _i32, _i64, _i32, _p, _p, _p, _p, _p, _p]),
     "mkv_paged_tree_workspace_bytes": (_sz, [_i32, _i64, _i32, _i32, _i32, _i32, _i32]),
     "mkv_paged_tree_attention": (ctypes.c_int, [
+        _p, _i64, _i64, _i32, _p, _p, _i32, _p, _p, _p, _p, _i64, _i32, _p, _i32, _i64, _i32, _p, _i32,
+        _p, _i32, _p, _i64, _i32, _i32, _i64, _i32, _i32, _i32, _f32, _p, _i64, _i64, _p, _sz, _p]),
+    "mkv_paged_tree_attention_zeroed": (ctypes.c_int, [
         _p, _i64, _i64, _i32, _p, _p, _i32, _p, _p, _p, _p, _i64, _i32, _p, _i32, _i64, _i32, _p, _i32,
         _p, _i32, _p, _i64, _i32, _i32, _i64, _i32, _i32, _i32, _f32, _p, _i64, _i64, _p, _sz, _p]),
     "mkv_tree_accept": (ctypes.c_int, [

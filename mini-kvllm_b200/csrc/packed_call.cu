@@ -28,7 +28,8 @@ extern "C" int mkv_call_packed(int32_t call, const int64_t* args) {
   if (!args) return set_error(MKV_ERR_INVALID_ARGUMENT, "mkv_call_packed: null pointer argument");
   Args x{args};
   switch (call) {
-    case MKV_CALL_PAGED_TREE_ATTENTION: {
+    case MKV_CALL_PAGED_TREE_ATTENTION:
+    case MKV_CALL_PAGED_TREE_ATTENTION + MKV_CALL_ZEROED: {
       const void* q = x.ptr<const void>();
       const int64_t qst = x.i64(), qsh = x.i64();
       const int32_t qdt = x.i32();
@@ -60,8 +61,9 @@ extern "C" int mkv_call_packed(int32_t call, const int64_t* args) {
       void* ws = x.ptr<void>();
       const size_t wsb = (size_t)x.i64();
       void* stream = x.ptr<void>();
-      return mkv_paged_tree_attention(q, qst, qsh, qdt, k, v, cdt, ks, vs, kss, vss, nb, bs, bt, btt, bts, maxb, cl, clt,
-                                      cu, cut, mask, mst, words, B, T, H, KVH, D, scale, out, ost, osh, ws, wsb, stream);
+      const auto fn = call & MKV_CALL_ZEROED ? mkv_paged_tree_attention_zeroed : mkv_paged_tree_attention;
+      return fn(q, qst, qsh, qdt, k, v, cdt, ks, vs, kss, vss, nb, bs, bt, btt, bts, maxb, cl, clt, cu, cut, mask, mst,
+                words, B, T, H, KVH, D, scale, out, ost, osh, ws, wsb, stream);
     }
     case MKV_CALL_TREE_METADATA:
     case MKV_CALL_TREE_ACCEPT: {

@@ -193,16 +193,48 @@ __global__ void __launch_bounds__(kGThreads) paged_tree_generic_kernel(const __g
 }
 
 // ============================================================ combine
+// Rows of no sequence (before row `first` and from row `last` on) become 0: threads tid of n, a warp
+// per row and head.
+template <typename QT>
+__device__ __noinline__ void zero_rows(const Params& p, int64_t first, int64_t last, int64_t tid, int64_t n) {
+  const int64_t rows = first + p.total_q - last;
+  const int lane = tid & 31;
+  for (int64_t i = tid >> 5; i < rows * p.num_heads; i += n >> 5) {
+    int64_t r = i / p.num_heads;
+    const int64_t h = i - r * p.num_heads;
+    if (r >= first) r += last - first;
+    QT* o = reinterpret_cast<QT*>(p.out) + r * p.o_st + h * p.o_sh;
+    for (int d = lane; d < p.head_dim; d += 32) o[d] = from_f32<QT>(0.0f);
+  }
+}
+
+template <typename QT>
+__global__ void __launch_bounds__(128) paged_tree_zero_kernel(const __grid_constant__ Params p) {
+  zero_rows<QT>(p, 0, 0, (int64_t)blockIdx.x * 128 + threadIdx.x, (int64_t)gridDim.x * 128);
+}
+
 // Joins the parts of each split unit: sum_i 2^(m_i - M) acc_i / sum_i 2^(m_i - M) l_i. CTA
 // (c, y) takes rows kCWarps y .. of the unit that desc[c] names, a warp per row: the lanes
 // read the parts' maxima and sums side by side, then the parts' rows in order. Four dependent loads
-// deep; 4 us behind a small call, 8 us for the 12 MB of parts of a full one.
+// deep; 4 us behind a small call, 8 us for the 12 MB of parts of a full one. The rows of no sequence
+// are this kernel's too where they are to be 0 (their number is known on the device alone).
 constexpr int kCWarps = 4;
 
 template <typename QT>
-__global__ void __launch_bounds__(32 * kCWarps) paged_tree_combine_kernel(const Params p, int RT) {
+__global__ void __launch_bounds__(32 * kCWarps) paged_tree_combine_kernel(const __grid_constant__ Params p, int RT) {
+  int64_t first = 0, last = p.total_q;  // rows of sequences
+  if (p.zero_rest) {
+    first = ld_idx(p.cu, p.cu_i64, 0);
+    last = ld_idx(p.cu, p.cu_i64, p.num_seqs);
+  }
   pdl_wait();
   const int4 d = p.desc[2 * blockIdx.x], e = p.desc[2 * blockIdx.x + 1];
+  if (first > 0 || last < p.total_q) {
+    first = min(max(first, (int64_t)0), p.total_q);
+    last = max(min(last, p.total_q), first);
+    zero_rows<QT>(p, first, last, ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * (32 * kCWarps) + threadIdx.x,
+                  (int64_t)gridDim.y * gridDim.x * (32 * kCWarps));
+  }
   const int parts_all = d.x, kvh = d.y;
   const int lane = threadIdx.x & 31, row = blockIdx.y * kCWarps + (threadIdx.x >> 5);
   const int R = d.z + row;
@@ -262,6 +294,15 @@ int launch_combine(const Params& p, int ctas, int rows, cudaStream_t s) {
   return cuda_status(cudaLaunchKernelEx(&cfg, paged_tree_combine_kernel<QT>, p, rows), "paged_tree_combine launch");
 }
 
+int launch_zero(const Params& p, int q_dtype, cudaStream_t s) {
+  const int64_t warps = p.total_q * p.num_heads, ctas = (warps + 3) / 4, most = 8 * kNumSMs;
+  const int grid = (int)(ctas < most ? ctas : most);
+  if (q_dtype == MKV_DTYPE_F16) paged_tree_zero_kernel<f16><<<grid, 128, 0, s>>>(p);
+  else if (q_dtype == MKV_DTYPE_BF16) paged_tree_zero_kernel<bf16><<<grid, 128, 0, s>>>(p);
+  else paged_tree_zero_kernel<float><<<grid, 128, 0, s>>>(p);
+  return cuda_status(cudaGetLastError(), "paged_tree_zero launch");
+}
+
 template <typename QT, typename CT>
 int launch_generic(const Params& p, cudaStream_t s) {
   const int bytes = (kGRows * p.head_dim + kGKT * (2 * p.head_dim + 4) + kGRows * kGKT + kGKT) * 4;
@@ -315,19 +356,27 @@ extern "C" size_t mkv_paged_tree_workspace_bytes(int32_t num_seqs, int64_t total
   return (head_dim == 128 || head_dim == 64) && q_dtype != MKV_DTYPE_F32 && tc > generic ? tc : generic;
 }
 
-extern "C" int mkv_paged_tree_attention(
-    const void* query, int64_t q_stride_token, int64_t q_stride_head, int32_t q_dtype,
-    const void* k_cache, const void* v_cache, int32_t cache_dtype, const float* k_scale,
-    const float* v_scale, const float* k_scales, const float* v_scales, int64_t num_blocks,
-    int32_t block_size, const void* block_tables, int32_t block_table_index_type,
-    int64_t block_table_stride_seq, int32_t max_num_blocks, const void* context_lens,
-    int32_t context_lens_index_type, const void* cu_seqlens_q, int32_t cu_seqlens_index_type,
-    const uint64_t* tree_mask, int64_t mask_stride_token, int32_t mask_words, int32_t num_seqs,
-    int64_t total_q, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim, float scale,
-    void* out, int64_t out_stride_token, int64_t out_stride_head, void* workspace,
-    size_t workspace_bytes, void* stream) {
+#define TREE_PARAMETERS \
+    const void* query, int64_t q_stride_token, int64_t q_stride_head, int32_t q_dtype, \
+    const void* k_cache, const void* v_cache, int32_t cache_dtype, const float* k_scale, \
+    const float* v_scale, const float* k_scales, const float* v_scales, int64_t num_blocks, \
+    int32_t block_size, const void* block_tables, int32_t block_table_index_type, \
+    int64_t block_table_stride_seq, int32_t max_num_blocks, const void* context_lens, \
+    int32_t context_lens_index_type, const void* cu_seqlens_q, int32_t cu_seqlens_index_type, \
+    const uint64_t* tree_mask, int64_t mask_stride_token, int32_t mask_words, int32_t num_seqs, \
+    int64_t total_q, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim, float scale, \
+    void* out, int64_t out_stride_token, int64_t out_stride_head, void* workspace, \
+    size_t workspace_bytes, void* stream
+#define TREE_ARGUMENTS \
+    query, q_stride_token, q_stride_head, q_dtype, k_cache, v_cache, cache_dtype, k_scale, v_scale, k_scales, \
+    v_scales, num_blocks, block_size, block_tables, block_table_index_type, block_table_stride_seq, \
+    max_num_blocks, context_lens, context_lens_index_type, cu_seqlens_q, cu_seqlens_index_type, tree_mask, \
+    mask_stride_token, mask_words, num_seqs, total_q, num_heads, num_kv_heads, head_dim, scale, out, \
+    out_stride_token, out_stride_head, workspace, workspace_bytes, stream
+
+namespace {
+int tree_attention(const char* fn, bool zero_rest, TREE_PARAMETERS) {
   clear_error();
-  const char* fn = "mkv_paged_tree_attention";
   if (num_seqs < 0 || total_q < 0 || num_heads <= 0 || num_kv_heads <= 0 || head_dim <= 0 || block_size <= 0 ||
       max_num_blocks < 0 || num_blocks < 0 || mask_words < 1)
     return set_error(MKV_ERR_INVALID_ARGUMENT, "%s: bad sizes", fn);
@@ -356,15 +405,16 @@ extern "C" int mkv_paged_tree_attention(
                      "%s: an 8-bit cache needs k_scale and v_scale, or k_scales and v_scales", fn);
   if (cache_dtype == MKV_DTYPE_INT8 && !row_scales)
     return set_error(MKV_ERR_INVALID_ARGUMENT, "%s: an INT8 cache needs k_scales and v_scales", fn);
-  if (num_seqs == 0 || total_q == 0) return MKV_OK;
-  if (!query || !out || !tree_mask || !context_lens || !cu_seqlens_q ||
-      (max_num_blocks > 0 && !block_tables) || (num_blocks > 0 && (!k_cache || !v_cache)))
+  if (total_q == 0 || (num_seqs == 0 && !zero_rest)) return MKV_OK;
+  if (num_seqs > 0 && (!query || !tree_mask || !context_lens || !cu_seqlens_q ||
+                       (max_num_blocks > 0 && !block_tables) || (num_blocks > 0 && (!k_cache || !v_cache))))
     return set_error(MKV_ERR_INVALID_ARGUMENT, "%s: null pointer argument", fn);
+  if (!out) return set_error(MKV_ERR_INVALID_ARGUMENT, "%s: null pointer argument", fn);
   if (((uintptr_t)k_cache | (uintptr_t)v_cache) & 15)
     return set_error(MKV_ERR_INVALID_ARGUMENT, "%s: caches must be 16-byte aligned", fn);
   const size_t need = mkv_paged_tree_workspace_bytes(num_seqs, total_q, num_heads, num_kv_heads, head_dim, q_dtype,
                                                      cache_dtype);
-  if (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15))
+  if (num_seqs > 0 && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15)))
     return set_error(MKV_ERR_WORKSPACE, "%s: needs a 16-byte aligned workspace of %zu bytes (got %zu)", fn, need,
                      workspace ? workspace_bytes : (size_t)0);
   tree::Params p = {};
@@ -400,6 +450,9 @@ extern "C" int mkv_paged_tree_attention(
   p.out = out;
   p.o_st = out_stride_token;
   p.o_sh = out_stride_head;
+  p.zero_rest = zero_rest;
+  cudaStream_t s = (cudaStream_t)stream;
+  if (num_seqs == 0) return tree::launch_zero(p, q_dtype, s);
   const tree::Plan plan = tree::tc_supported(p, q_dtype, cache_dtype)
                               ? tree::Plan{true, tree::kTcRows, kNumSMs}
                               : tree::Plan{false, tree::kGRows, tree::kGCtas};
@@ -408,10 +461,17 @@ extern "C" int mkv_paged_tree_attention(
   p.part_acc = (float*)((char*)workspace + w.acc);
   p.part_ml = (float2*)((char*)workspace + w.ml);
   p.desc = (int4*)((char*)workspace + w.desc);
-  cudaStream_t s = (cudaStream_t)stream;
   switch (q_dtype) {
     case MKV_DTYPE_F16: return tree::run<f16>(p, plan, q_dtype, cache_dtype, s);
     case MKV_DTYPE_BF16: return tree::run<bf16>(p, plan, q_dtype, cache_dtype, s);
     default: return tree::run<float>(p, plan, q_dtype, cache_dtype, s);
   }
+}
+}  // namespace
+
+extern "C" int mkv_paged_tree_attention(TREE_PARAMETERS) {
+  return tree_attention("mkv_paged_tree_attention", false, TREE_ARGUMENTS);
+}
+extern "C" int mkv_paged_tree_attention_zeroed(TREE_PARAMETERS) {
+  return tree_attention("mkv_paged_tree_attention_zeroed", true, TREE_ARGUMENTS);
 }

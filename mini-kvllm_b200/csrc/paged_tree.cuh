@@ -33,6 +33,7 @@ struct Params {
   const float* v_scales;
   void* out;
   int64_t o_st, o_sh;  // elements
+  bool zero_rest;      // rows of no sequence become 0 (otherwise they are left)
   // split units: partial sums (2 slots per CTA) and one descriptor per CTA
   float* part_acc;  // [slot][row][head_dim], relative to the row's partial maximum
   float2* part_ml;  // [slot][row] = (maximum in the exp2 domain, sum)

@@ -586,8 +586,8 @@ def paged_attention_tree(query: torch.Tensor, k_cache: torch.Tensor, v_cache: to
     of its context_lens[b] cached ones. A row sees every token before the sequence's nodes,
     and node j when bit j % 64 of its word tree_mask[row, j // 64] (int64, as tree_metadata
     makes it) is set. Returns (total_q, num_heads, head_dim) in the query dtype; a row that
-    sees nothing is 0, and rows of no sequence (a padded batch's) are not written: with
-    `out` given they keep what it held. Caches and scales as for paged_attention_prefill.
+    sees nothing is 0, and so are the rows of no sequence (a padded batch's), which keep what
+    they held where `out` is given. Caches and scales as for paged_attention_prefill.
     Not in the reference, which decodes one token per sequence and step."""
     fn = "paged_attention_tree"
     if query.dim() != 3 or query.shape[1] != num_heads or query.shape[2] != head_dim:
@@ -641,7 +641,7 @@ def paged_attention_tree(query: torch.Tensor, k_cache: torch.Tensor, v_cache: to
         output = out
     else:
         output = torch.empty_like(query) if query.is_contiguous() else query.new_empty(query.shape)
-    if total_q == 0 or num_seqs == 0:
+    if total_q == 0 or (num_seqs == 0 and out is not None):
         return output
     qs = query.stride()
     if qs[2] != 1:
@@ -663,7 +663,8 @@ def paged_attention_tree(query: torch.Tensor, k_cache: torch.Tensor, v_cache: to
     # from the caching allocator at each call: calls on other streams, and captured graphs,
     # never share a workspace
     ws = query.new_empty(ws_n, dtype=torch.uint8)
-    st = _call_packed(lib, idx, _lib.CALL_PAGED_TREE_ATTENTION, _lib.PACK_TREE_ATTENTION, (
+    call = _lib.CALL_PAGED_TREE_ATTENTION + (_lib.CALL_ZEROED if out is None else 0)
+    st = _call_packed(lib, idx, call, _lib.PACK_TREE_ATTENTION, (
         query.data_ptr(), qs[0], qs[1], dt, k_cache.data_ptr(), v_cache.data_ptr(), cache_code, kp, vp,
         kps, vps, num_blocks, block_size, block_tables.data_ptr(), _INDEX[block_tables.dtype], bs[0],
         block_tables.shape[1], lens.data_ptr(), _INDEX[lens.dtype], cu.data_ptr(), _INDEX[cu.dtype],

@@ -460,3 +460,91 @@ def test_a_context_without_the_field(attn, monkeypatch):
     context = types.SimpleNamespace(is_prefill=False, slot_mapping=None, context_lens=c.lens, block_tables=c.bt)
     monkeypatch.setattr(attn, "get_context", lambda: context)
     c.check(layer(c.q, None, None).view(2, 8, 128))
+
+
+def stale(*shape, dtype):
+    """Leaves NaN in the memory that the next tensors of this size are likely to get."""
+    held = [torch.full(shape, float("nan"), dtype=dtype, device=DEV) for _ in range(4)]
+    torch.cuda.synchronize()
+    del held
+
+
+@pytest.mark.parametrize("dtype,mode,D", [(BF16, "auto", 128), (F16, "auto", 64), (F32, "auto", 128),
+                                          (BF16, "fp8_per_tensor", 128), (F16, "int8_per_token_head", 64),
+                                          (BF16, "auto", 80)])
+@pytest.mark.parametrize("front,behind", [(0, 5), (3, 0), (2, 300), (0, 0)])
+def test_rows_of_no_sequence_are_zero_without_out(attn, dtype, mode, D, front, behind):
+    """A padded batch's rows, before the first and behind the last sequence, are defined: zeros,
+    whatever their queries and masks hold, and whatever the memory held."""
+    c = Case(27, [50, 0, 2100], [4, 0, 6], 8, 2, D, 16, dtype, mode)
+    nan = lambda n: torch.full((n, 8, D), float("nan"), device=DEV, dtype=dtype)  # noqa: E731
+    ones = lambda n: torch.full((n, c.words), -1, device=DEV, dtype=torch.int64)  # noqa: E731
+    q, mask = torch.cat([nan(front), c.q, nan(behind)]), torch.cat([ones(front), c.mask, ones(behind)])
+    cu = c.cut
+    c.mask, c.cut = mask, cu + front
+    stale(*q.shape, dtype=dtype)
+    got = c.run(attn, q=q)
+    c.cut = cu
+    c.check(got[front:front + 10])
+    assert (got[:front] == 0).all() and (got[front + 10:] == 0).all()
+    out = torch.full((front + 10 + behind, 9, D + 2), 7.0, dtype=dtype, device=DEV)  # a given `out` keeps its rows
+    c.cut = cu + front
+    c.run(attn, q=q, out=out[:, 1:, :D])
+    c.cut = cu
+    c.check(out[front:front + 10, 1:, :D])
+    assert (out[:front] == 7).all() and (out[front + 10:] == 7).all()
+
+
+def test_padding_alone_is_zero(attn):
+    """A captured step whose every row is padding (no sequence)."""
+    q = torch.full((9, 8, 128), float("nan"), dtype=BF16, device=DEV)
+    cache = torch.zeros(3, 16, 2, 128, dtype=BF16, device=DEV)
+    none = torch.zeros(0, dtype=torch.int64, device=DEV)
+    stale(9, 8, 128, dtype=BF16)
+    got = attn.paged_attention_tree(q, cache, cache, torch.zeros(0, 4, dtype=torch.int32, device=DEV), none,
+                                    torch.zeros(1, dtype=torch.int32, device=DEV),
+                                    torch.zeros(9, 1, dtype=torch.int64, device=DEV), 0.1, 8, 2, 128, 16)
+    assert (got == 0).all()
+
+
+@pytest.mark.parametrize("captured", [False, True])
+def test_a_padded_step_through_two_layers(attn, captured):
+    """Attention.forward on a padded tree step: what its padding rows hand to the next layer is
+    finite, so that layer's append, which takes its e4m3 scale from all rows of its first step,
+    padding included, does not take it from whatever memory held."""
+    c = Case(28, [100, 30], [6, 9], 8, 2, 128, 16, BF16, poison=False)
+    ctx, kv = mkv_module("utils.context"), mkv_module("engine.kv_cache")
+    cache = kv.allocate_kv_cache(2, c.k.shape[0], 16, 2, 128, "fp8_per_tensor", BF16, DEV)
+    layers = [attn.Attention(8, 128, 1.0, 2, 16) for _ in range(2)]
+    kv.bind_kv_cache(layers, cache)
+    pad = 4
+    parents = torch.tensor([-1, 0, 0, 1, 1, 4] + [-1] + list(range(8)) + [-1] * pad, dtype=torch.int32, device=DEV)
+    q = torch.cat([c.q, torch.ones(pad, 8, 128, dtype=BF16, device=DEV)])
+    prefix = c.lens - torch.tensor([6, 9], device=DEV)
+
+    def step():
+        m = kv.tree_metadata(parents, c.cut, prefix, c.bt, 16, 9)
+        ctx.set_context(True, cu_seqlens_q=c.cut, slot_mapping=m.slot_mapping, context_lens=m.context_lens,
+                        block_tables=c.bt, positions=m.positions, tree_mask=m.tree_mask)
+        x = layers[0](q, q[:, :2], q[:, 2:4])
+        y = layers[1](x.view(-1, 8, 128), x.view(-1, 8, 128)[:, :2], x.view(-1, 8, 128)[:, 2:4])
+        return x, y
+
+    try:
+        if captured:
+            step()
+            cache.k_scale.fill_(1.0), cache.v_scale.fill_(1.0)
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                x, y = step()
+            x.fill_(float("nan")), y.fill_(float("nan"))
+            graph.replay()
+        else:
+            stale(19, 8, 128, dtype=BF16)
+            x, y = step()
+        torch.cuda.synchronize()
+    finally:
+        ctx.reset_context()
+    assert (x[15:] == 0).all() and (y[15:] == 0).all()
+    assert torch.isfinite(x).all() and torch.isfinite(y).all()
+    assert torch.isfinite(cache.k_scale).all() and torch.isfinite(cache.v_scale).all()

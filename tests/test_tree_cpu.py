@@ -182,3 +182,22 @@ def test_the_roles_of_a_kernel_meet_at_bounded_barriers_only():
         assert not re.search(r"__barrier_sync|named_barrier|cuda::barrier", code), f.name
         waits = [m.start() for m in re.finditer(r"mbarrier\.try_wait|mbarrier\.test_wait", code)]
         assert len(waits) == (1 if f.name == "sm100.cuh" else 0), f.name
+
+
+def test_the_zeroed_variant_refuses_the_same():
+    """mkv_paged_tree_attention_zeroed, and the packed call of it."""
+    lib = lib_mod.load()
+    words = dict(q=P, qst=1024, qsh=128, qdt=2, k=P, v=P, cdt=2, ks=0, vs=0, kss=0, vss=0, nb=10, bs=16, bt=P, btt=0,
+                 btst=8, maxb=8, cl=P, clt=1, cu=P, cut=0, mask=P, mst=1, words=1, B=2, T=9, H=8, KVH=2, D=128, scale=0.1,
+                 out=P, ost=1024, osh=128, ws=P, wsb=1 << 40, stream=0)
+    for kw, status in ((dict(H=7), 1), (dict(D=100), 2), (dict(mask=0), 1), (dict(out=0), 1), (dict(B=0, out=0), 1),
+                       (dict(wsb=10), 3), (dict(B=0, k=P + 8), 1), (dict(T=0, out=0), 0)):
+        a = {**words, **kw}
+        packed = lib.mkv_call_packed(lib_mod.CALL_PAGED_TREE_ATTENTION + lib_mod.CALL_ZEROED,
+                                     lib_mod.PACK_TREE_ATTENTION(*a.values()))
+        message = lib.mkv_last_error()
+        assert packed == lib.mkv_paged_tree_attention_zeroed(*[v or None if type(v) is int and n in (
+            "q", "k", "v", "ks", "vs", "kss", "vss", "bt", "cl", "cu", "mask", "out", "ws", "stream") else v
+            for n, v in a.items()]) == status
+        assert message == lib.mkv_last_error() and (status == 0 or b"mkv_paged_tree_attention_zeroed" in message)
+    assert lib.mkv_call_packed(lib_mod.CALL_MOVE_KV_ROWS + lib_mod.CALL_ZEROED, b"\0" * 400) == 1
