@@ -527,7 +527,12 @@ MKV_API int mkv_tree_metadata(const void* parents, int32_t parents_index_type, c
  * (head_dim contiguous). workspace: 16-byte aligned, at least
  * mkv_paged_tree_workspace_bytes(...), its contents on entry do not matter; calls that may
  * overlap on the GPU need workspaces of their own.
+ * The warps of a thread block hand tiles to each other and wait no longer than a limit for one;
+ * a block that meets it makes every row that it has a part in NaN. mkv_set_wait_limit sets the
+ * limit for the calls that follow, in GPU clocks, and returns the last one (2e9, about a second,
+ * where none was set; a debugger that stops single warps needs more; 0 lets no wait succeed).
  */
+MKV_API int64_t mkv_set_wait_limit(int64_t clocks);
 MKV_API size_t mkv_paged_tree_workspace_bytes(int32_t num_seqs, int64_t total_q, int32_t num_heads,
                                               int32_t num_kv_heads, int32_t head_dim, int32_t q_dtype,
                                               int32_t cache_dtype);

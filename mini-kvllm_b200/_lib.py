@@ -75,6 +75,7 @@ SIGNATURES: dict[str, tuple] = {
     "mkv_decode_metadata": (ctypes.c_int, [_p, _i32, _i32, _i32, _p, _p, _p]),
     "mkv_tree_metadata": (ctypes.c_int, [
         _p, _i32, _p, _i32, _p, _i32, _p, _i32, _i64, _i32, _i32, _i32, _i64, _i32, _p, _p, _p, _p, _p, _p]),
+    "mkv_set_wait_limit": (_i64, [_i64]),
     "mkv_paged_tree_workspace_bytes": (_sz, [_i32, _i64, _i32, _i32, _i32, _i32, _i32]),
     "mkv_paged_tree_attention": (ctypes.c_int, [
         _p, _i64, _i64, _i32, _p, _p, _i32, _p, _p, _p, _p, _i64, _i32, _p, _i32, _i64, _i32, _p, _i32,

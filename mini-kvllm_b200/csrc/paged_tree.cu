@@ -10,7 +10,10 @@
 //
 // All query rows of a kv head (nodes x GQA group) share each K/V tile, and the token axis
 // is split evenly over the CTAs (paged_tree.cuh), so K and V are read about once.
+#include <atomic>
+
 #include "paged_tree.cuh"
+#include "sm100.cuh"
 
 namespace mkv {
 namespace tree {
@@ -329,7 +332,10 @@ int run(const Params& p, const Plan& plan, int q_dtype, int cache_dtype, cudaStr
   return st == MKV_OK ? launch_combine<QT>(p, plan.ctas, plan.rows, s) : st;
 }
 
+std::atomic<int64_t> g_wait_limit{sm100::kWaitCycles};
 }  // namespace
+
+int64_t wait_limit() { return g_wait_limit.load(std::memory_order_relaxed); }
 
 Workspace workspace(int ctas, int rows, int head_dim) {
   auto up = [](size_t x) { return (x + 255) / 256 * 256; };
@@ -354,6 +360,10 @@ extern "C" size_t mkv_paged_tree_workspace_bytes(int32_t num_seqs, int64_t total
   const size_t generic = tree::workspace(tree::kGCtas, tree::kGRows, head_dim).total;
   const size_t tc = tree::workspace(kNumSMs, tree::kTcRows, head_dim).total;
   return (head_dim == 128 || head_dim == 64) && q_dtype != MKV_DTYPE_F32 && tc > generic ? tc : generic;
+}
+
+extern "C" int64_t mkv_set_wait_limit(int64_t clocks) {
+  return tree::g_wait_limit.exchange(clocks < 0 ? 0 : clocks, std::memory_order_relaxed);
 }
 
 #define TREE_PARAMETERS \
@@ -451,6 +461,7 @@ int tree_attention(const char* fn, bool zero_rest, TREE_PARAMETERS) {
   p.o_st = out_stride_token;
   p.o_sh = out_stride_head;
   p.zero_rest = zero_rest;
+  p.wait_limit = tree::wait_limit();
   cudaStream_t s = (cudaStream_t)stream;
   if (num_seqs == 0) return tree::launch_zero(p, q_dtype, s);
   const tree::Plan plan = tree::tc_supported(p, q_dtype, cache_dtype)

@@ -26,6 +26,7 @@ struct Params {
   int num_seqs, num_heads, num_kv_heads, head_dim, group;
   int64_t total_q;
   int unit_cost;  // of the schedule, in token tiles
+  long long wait_limit;  // clocks that a wait may take
   float qk_scale_log2;
   const float* k_scale;   // per-tensor scales of e4m3 pages, or null
   const float* v_scale;
@@ -277,11 +278,39 @@ __device__ __forceinline__ int slot_of(const Unit& u, int c) {
 // part has a finite one), as opposed to a row that saw nothing (0).
 constexpr float kSeenInf = -1.0f;
 
+// What a CTA gives when one of its waits has run out: NaN in every row of its share (in the partial
+// sums of the units that it has a part of, which the join carries into the rows). Block-collective,
+// called when nothing of the CTA is in flight any more; red as for begin().
+template <int RT, int KT, int NT, typename QT>
+__device__ __noinline__ void give_up(const Params& p, long long* red) {
+  Walk w;
+  if (!begin<RT, KT, NT>(p, blockIdx.x, gridDim.x, red, w)) return;
+  Unit u;
+  while (next<RT, KT>(p, w, u)) {
+    const int rows = (int)min((int64_t)RT, (int64_t)u.s.nodes * p.group - (int64_t)u.mt * RT);
+    const int slot = slot_of(u, blockIdx.x);
+    for (int r = threadIdx.x >> 5; r < rows; r += NT / 32) {  // a warp per row
+      const int lane = threadIdx.x & 31;
+      if (slot >= 0) {
+        if (lane == 0) p.part_ml[(int64_t)slot * RT + r] = make_float2(-INFINITY, NAN);
+        continue;
+      }
+      const int R = u.mt * RT + r, node = R / p.group;
+      QT* o = reinterpret_cast<QT*>(p.out) + (u.s.q0 + node) * p.o_st +
+              (int64_t)(u.kvh * p.group + R - node * p.group) * p.o_sh;
+      for (int d = lane; d < p.head_dim; d += 32) o[d] = from_f32<QT>(NAN);
+    }
+  }
+}
+
 // ---------------------------------------------------------------- host side
 struct Workspace {
   size_t acc, ml, desc, total;  // offsets and size in bytes
 };
 Workspace workspace(int ctas, int rows, int head_dim);
+
+// Clocks that a wait in the kernels may take (mkv_set_wait_limit).
+int64_t wait_limit();
 
 // tcgen05 variant (paged_tree_tc.cu): whether it takes the call, and its launch.
 constexpr int kTcRows = 128;

@@ -31,8 +31,9 @@
 // and others do not, are searched for infinities and NaN: those are zeroed too, and added in
 // at the end to the rows that see them.
 //
-// Every wait is bounded (sm100::kWaitCycles); a role that gives up raises the abort flag, the
-// others stop, loads and MMAs in flight are waited for and TMEM is freed.
+// Every wait is bounded (mkv_set_wait_limit); a role that gives up raises the abort flag, the
+// others stop, loads and MMAs in flight are waited for, TMEM is freed, and the CTA's rows become
+// NaN (give_up), so that the failure is seen.
 #include <cuda.h>
 
 #include <type_traits>
@@ -78,8 +79,8 @@ struct Layout {
 
 // A wait that has not been met at once; out of line, as the roles' code should stay small
 // (instructions that one role fetches push out another's).
-__device__ __noinline__ bool wait_on(uint64_t* bar, uint32_t parity, const volatile int* abort) {
-  return mbar_wait(bar, parity, abort);
+__device__ __noinline__ bool wait_on(uint64_t* bar, uint32_t parity, const volatile int* abort, long long limit) {
+  return mbar_wait(bar, parity, abort, limit);
 }
 
 // 16 bytes of an 8-bit row -> 16 f16 values, exact.
@@ -209,7 +210,7 @@ paged_tree_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ C
   const int nseg = kTile / seg_rows;
   auto wait = [&](uint64_t* bar, uint32_t phase) -> bool {  // warp-uniform
     bool done = mbar_try_wait(bar, phase & 1);
-    if (!done) done = wait_on(bar, phase & 1, abort_flag);
+    if (!done) done = wait_on(bar, phase & 1, abort_flag, p.wait_limit);
     return __all_sync(0xffffffffu, done);
   };
   const int bs_log2 = 31 - __clz(p.block_size);
@@ -224,7 +225,7 @@ paged_tree_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ C
   Unit u = {};
   uint32_t g = 0;     // tiles of this CTA before the unit's
   uint32_t unit = 0;  // units before this one
-  bool ok = true;
+  bool ok = p.wait_limit > 0;  // (0: no wait is allowed at all)
 
   if (warp == 0) {
     // ================================================================ producer
@@ -813,6 +814,7 @@ paged_tree_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ C
   __syncthreads();
   tc_fence_after_sync();
   if (warp == 1) tmem_dealloc(tmem, kTmemCols);
+  if (*abort_flag) give_up<kRows, kTile, L::kThreads, QT>(p, reinterpret_cast<long long*>(smem + L::K0));
 }
 
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,

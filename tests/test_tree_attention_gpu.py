@@ -548,3 +548,31 @@ def test_a_padded_step_through_two_layers(attn, captured):
     assert (x[15:] == 0).all() and (y[15:] == 0).all()
     assert torch.isfinite(x).all() and torch.isfinite(y).all()
     assert torch.isfinite(cache.k_scale).all() and torch.isfinite(cache.v_scale).all()
+
+
+@pytest.mark.parametrize("dtype,mode,D", [(BF16, "auto", 128), (F16, "auto", 64), (BF16, "fp8_per_tensor", 128),
+                                          (BF16, "fp8_per_token_head", 64), (F16, "int8_per_token_head", 128)])
+@pytest.mark.parametrize("prefix,nodes", [([411], [8]), ([9000, 3, 0, 700], [33, 0, 1, 20]), ([40] * 200, [3] * 200)])
+def test_waits_that_run_out_are_seen(attn, dtype, mode, D, prefix, nodes):
+    """With a limit of 0 every block gives up before its first wait, with nothing in flight: the
+    call ends, all rows of sequences are NaN (split and whole units, over finite values of earlier
+    calls in the workspace and the output), other rows are what they are without that, and the
+    next call, with the limit as it was, is right."""
+    lib = mkv_module("_lib").load()
+    c = Case(29, prefix, nodes, 8, 2, D, 16, dtype, mode)
+    total = c.cu[-1]
+    q = torch.cat([c.q, torch.ones(3, 8, D, dtype=dtype, device=DEV)])
+    c.mask = torch.cat([c.mask, torch.zeros(3, c.words, dtype=torch.int64, device=DEV)])
+    out = torch.full((total + 3, 8, D), 5.0, dtype=dtype, device=DEV)
+    c.run(attn, q=q, out=out)  # leaves finite partial sums where the next call's workspace will be
+    c.check(out[:total])
+    was = lib.mkv_set_wait_limit(0)
+    try:
+        given, own = c.run(attn, q=q, out=out.clone()), c.run(attn, q=q)
+        torch.cuda.synchronize()
+    finally:
+        assert lib.mkv_set_wait_limit(was) == 0
+    assert torch.isnan(given[:total]).all() and (given[total:] == 5).all()
+    assert torch.isnan(own[:total]).all() and (own[total:] == 0).all()
+    again = c.run(attn, q=q, out=out)
+    c.check(again[:total])

@@ -201,3 +201,12 @@ def test_the_zeroed_variant_refuses_the_same():
             for n, v in a.items()]) == status
         assert message == lib.mkv_last_error() and (status == 0 or b"mkv_paged_tree_attention_zeroed" in message)
     assert lib.mkv_call_packed(lib_mod.CALL_MOVE_KV_ROWS + lib_mod.CALL_ZEROED, b"\0" * 400) == 1
+
+
+def test_the_limit_of_waits():
+    lib = lib_mod.load()
+    first = lib.mkv_set_wait_limit(123)
+    assert first == 2_000_000_000
+    assert lib.mkv_set_wait_limit(-5) == 123  # below 0 counts as 0
+    assert lib.mkv_set_wait_limit(first) == 0
+    assert lib.mkv_set_wait_limit(first) == first
