@@ -50,6 +50,8 @@ constexpr int kRows = kTcRows, kTile = 128;
 constexpr int BLK = 128 * 128;  // 128 rows x 128 bytes: 64 columns of a 16-bit tile
 constexpr uint32_t kTmemCols = 512, kOCol = 256;
 constexpr int kSickSlots = 4;
+constexpr int kWide = 6;     // binades of V scales in a tile beyond which a row takes an exponent of its own
+constexpr float kHold = 60;  // binades that O may lie above its unit
 
 // kByte: 8-bit cache; kTok: with per-(token, head) scales.
 template <bool kByte, bool kTok, int kD>
@@ -71,7 +73,7 @@ struct Layout {
   static constexpr int ONE0 = QE0 + (kByte ? 2 * kRows : 0);          // [128] ones: K scales of a masked tile
   static constexpr int BAR0 = ONE0 + (kTok ? kTile * 4 : 0);
   static constexpr int NBAR = 2 * kKS + 2 * kVS + 2 * kRS + 4 + 2 + 2 + 1 + 2 + 1 + 1;
-  static constexpr int MISC0 = BAR0 + NBAR * 8;              // tmem base, abort, sick[4], exponents[2], maxima[2][4]
+  static constexpr int MISC0 = BAR0 + NBAR * 8;              // tmem base, abort, sick[4], exponents[2], ranges[2][4]
   static constexpr int BYTES = MISC0 + 64;
   static_assert(BYTES <= 232448, "shared memory per CTA");
   static_assert(kBeginWords(kThreads) * 8 <= TILE, "the schedule's scratch lies in the first K stage");
@@ -158,7 +160,7 @@ paged_tree_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ C
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::MISC0 + 4);
   volatile int* sick_s = reinterpret_cast<volatile int*>(smem + L::MISC0 + 8);
   volatile int* vexp_s = reinterpret_cast<volatile int*>(smem + L::MISC0 + 8 + 4 * kSickSlots);
-  volatile float* vmax_s = reinterpret_cast<volatile float*>(smem + L::MISC0 + 16 + 4 * kSickSlots);
+  volatile uint32_t* vmax_s = reinterpret_cast<volatile uint32_t*>(smem + L::MISC0 + 16 + 4 * kSickSlots);
   int8_t* qexp_s = reinterpret_cast<int8_t*>(smem + L::QE0);
   float* scales_s = reinterpret_cast<float*>(smem + L::SC0);
   float* ones_s = reinterpret_cast<float*>(smem + L::ONE0);
@@ -453,7 +455,8 @@ paged_tree_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ C
       }
       if (sc < 1e-37f) sc = 1e-37f;  // not 0, so that a masked -inf stays one
       float m = -INFINITY, l = 0.0f;  // reference (exp2 domain) and sum of this stream
-      int vexp = 0;                   // O holds values times 2^-vexp (kTok)
+      // kTok: O holds values times 2^-vexp, its terms so far are below 2^hold times their number
+      float vexp = 0.0f, hold = -INFINITY;
       bool seen = false;
       Entry next_e = seg_entry(u, u.k0 + stream);
 #pragma unroll 1
@@ -488,15 +491,12 @@ paged_tree_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ C
         if (kByte && (kTok || special)) {  // the converters have written the tile's scales and flags
           if (!(ok = wait(&vfull[st], vph))) break;
         }
+        float tile_exp = 0.0f, er = 0.0f;  // unit of the tile's V factors, and of this row's products
+        bool wide = false;
         if constexpr (kTok) {
           const int e = vexp_s[st];
-          if (e != vexp) {
-            if (ns != 0) {
-              alpha = exp2f((float)(vexp - e));
-              rescale = true;
-            }
-            vexp = e;
-          }
+          tile_exp = er = (float)(e >> 1);
+          wide = e & 1;
         }
         if (warp_live) {
           // 32 scores, times the tokens' K scales
@@ -547,36 +547,74 @@ paged_tree_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ C
           const bool need = mt > m + 8.0f;
           const float m_new = need ? mt : m;
           const float a2 = need ? exp2f(m - m_new) : 1.0f;  // 0 when m was -inf
+          if constexpr (kTok) {
+            // The tile's V factors are below 2, but where some are far below (wide) those that the row
+            // does not see, or that hardly weigh, must not push its products into the subnormals of f16:
+            // its own unit puts the largest product near 2^kBias. O may end up to 2^kHold above that.
+            if (wide) {
+              float top = -INFINITY;  // log2 of the largest weight times factor, rounded up
+#pragma unroll 1
+              for (int h = 0; h < 4; ++h) {
+                float v[32];
+                scores(h, v);
+#pragma unroll
+                for (int e = 0; e < 32; ++e) {
+                  const int fx = (int)(__float_as_uint(ksp[kTile + 32 * h + e]) >> 23 & 255u) - 126;
+                  top = fmaxf(top, fmaf(v[e], sc, (float)fx));
+                }
+              }
+              er = top == -INFINITY ? vexp : er + fminf(fmaxf(floorf(top - m_new), -120.0f), 120.0f);
+            }
+            if (need) hold -= m_new - m;
+            er = fmaxf(er, hold - kHold);
+            hold = fmaxf(hold, er);
+            alpha = exp2f(vexp - er + (need ? m - m_new : 0.0f));
+            rescale = vexp != er;
+            vexp = er;
+          }
           const float nref = kBias - (m_new == -INFINITY ? 0.0f : m_new);
           const uint64_t sc2 = f2_pack(sc, sc), nref2 = f2_pack(nref, nref);
           uint64_t acc[2] = {f2_pack(0.0f, 0.0f), f2_pack(0.0f, 0.0f)};
+          // (own: the row's unit is not the tile's)
+          auto weights = [&](auto own, float factor) {
 #pragma unroll 1
-          for (int h = 0; h < 4; ++h) {
-            float v[32];
-            uint32_t w[16];
-            scores(h, v);
+            for (int h = 0; h < 4; ++h) {
+              float v[32];
+              uint32_t w[16];
+              scores(h, v);
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              float x0, x1;
-              f2_unpack(f2_fma(f2_pack(v[2 * e], v[2 * e + 1]), sc2, nref2), x0, x1);
-              float p0 = ex2_approx(x0), p1 = ex2_approx(x1);  // 0 where masked
-              acc[e & 1] = f2_add(acc[e & 1], f2_pack(p0, p1));
-              if constexpr (kTok) {
-                const float2 f = *reinterpret_cast<const float2*>(ksp + kTile + 32 * h + 2 * e);
-                p0 *= f.x;
-                p1 *= f.y;
+              for (int e = 0; e < 16; ++e) {
+                float x0, x1;
+                f2_unpack(f2_fma(f2_pack(v[2 * e], v[2 * e + 1]), sc2, nref2), x0, x1);
+                float p0 = ex2_approx(x0), p1 = ex2_approx(x1);  // 0 where masked
+                acc[e & 1] = f2_add(acc[e & 1], f2_pack(p0, p1));
+                if constexpr (kTok) {
+                  float2 f = *reinterpret_cast<const float2*>(ksp + kTile + 32 * h + 2 * e);
+                  if constexpr (decltype(own)::value) {
+                    f.x *= factor;
+                    f.y *= factor;
+                  }
+                  p0 *= f.x;
+                  p1 *= f.y;
+                }
+                w[e] = pack2<MT>(p0, p1);
               }
-              w[e] = pack2<MT>(p0, p1);
+              tmem_st16u(sa + 16 * h, w);  // over columns of S that have been read
             }
-            tmem_st16u(sa + 16 * h, w);  // over columns of S that have been read
-          }
+          };
+          if (kTok && __any_sync(0xffffffffu, er != tile_exp))
+            weights(std::true_type{}, exp2f(fminf(fmaxf(tile_exp - er, -126.0f), 120.0f)));
+          else
+            weights(std::false_type{}, 1.0f);
           float s0, s1, s2, s3;
           f2_unpack(acc[0], s0, s1);
           f2_unpack(acc[1], s2, s3);
           const float sum = (s0 + s1) + (s2 + s3);
           if (i > stream) {  // O holds something
-            rescale |= __any_sync(0xffffffffu, need);
-            alpha *= a2;
+            rescale = __any_sync(0xffffffffu, rescale || need);
+            if constexpr (!kTok) alpha = a2;
+          } else {
+            rescale = false;
           }
           m = m_new;
           l = fmaf(l, a2, sum);
@@ -619,7 +657,7 @@ paged_tree_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ C
       tc_fence_after_sync();
       // the products of this unit are done with its Q: its buffer takes the statistics
       float4* stats = reinterpret_cast<float4*>(smem + L::Q0 + (unit & 1) * TILE);
-      stats[stream * kRows + rt] = make_float4(m, l, (float)vexp, seen ? 1.0f : 0.0f);
+      stats[stream * kRows + rt] = make_float4(m, l, vexp, seen ? 1.0f : 0.0f);
       __syncwarp();
       if (lane == 0) mbar_arrive(&xbar[0]);
       if (!(ok = wait(&xbar[0], unit))) break;
@@ -636,8 +674,8 @@ paged_tree_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ C
         const float lm = stream == 0 || both ? am * l : 0.0f, lx = stream == 1 || both ? ax * x[1] : 0.0f;
         float Ls = lm + lx;
         const bool any = seen || x[3] != 0.0f;
-        const float a0 = vs0 * (stream == 0 ? am * exp2f((float)vexp) : ax * exp2f(x[2]));
-        const float a1 = vs0 * (stream == 1 ? am * exp2f((float)vexp) : ax * exp2f(x[2]));
+        const float a0 = vs0 * (stream == 0 ? am * exp2f(vexp) : ax * exp2f(x[2]));
+        const float a1 = vs0 * (stream == 1 ? am * exp2f(vexp) : ax * exp2f(x[2]));
         const int slot = slot_of(u, blockIdx.x);
         float inv = 1.0f;
         if (slot < 0) inv = Ls == 0.0f ? (any ? NAN : 0.0f) : 1.0f / Ls;
@@ -774,28 +812,38 @@ paged_tree_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ C
           sick = clear_sick<0x7c00u>(smem + L::V0 + sv * TILE + r * 128, kD * 2);
         if constexpr (kTok) {
           // P takes the token's V scale times 2^-vexp: a power of two that follows the largest
-          // scale of a tile, moved only when that grows past it or falls 4 binades below
+          // scale of a tile, moved only when that grows past it or falls 4 binades below. Where the
+          // smallest lies far below the largest, the rows are told to take a unit of their own.
           if (node && !isfinite(vs)) {
             vs = 0.0f;
             sick = true;
           }
-          const float wm = warp_max(isfinite(vs) ? fabsf(vs) : 0.0f);
-          volatile float* mx = vmax_s + 4 * (k & 1);  // two sets: the other one may still be read
+          const uint32_t ex = (__float_as_uint(vs) >> 23) & 255u;  // the scale's exponent
+          const bool counts = ex != 0u && ex != 255u;
+          const uint32_t wm = __reduce_max_sync(0xffffffffu, counts ? ex : 0u) |
+                              __reduce_min_sync(0xffffffffu, counts ? ex : 255u) << 8;
+          volatile uint32_t* mx = vmax_s + 4 * (k & 1);  // two sets: the other one may still be read
           if (lane == 0) {
             mx[warp - 12] = wm;
             mbar_arrive(cbar);
           }
           __syncwarp();
           if (!(ok = wait(cbar, k))) break;  // (bounded as every wait: another converter may have given up)
-          const float tm = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-          if (tm > 0.0f) {
-            const int e = min(max((int)(__float_as_uint(tm) >> 23) - 127, -100), 100);
+          int top = 0, low = 255;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const uint32_t x = mx[j];
+            top = max(top, (int)(x & 255u));
+            low = min(low, (int)(x >> 8));
+          }
+          if (top > 0) {
+            const int e = min(top - 127, 126);
             if (e > vexp || e < vexp - 4) vexp = e;
           }
           float* out = scales_s + sv * 2 * kTile;
           out[r] = ks;
           out[kTile + r] = vs * pow2f(-vexp);
-          if (r == 0) vexp_s[sv] = vexp;
+          if (r == 0) vexp_s[sv] = 2 * vexp + (top > low + kWide);
         }
         if (sick) sick_s[unit % kSickSlots] = (int)unit + 1;
         fence_proxy_async_smem();

@@ -576,3 +576,55 @@ def test_waits_that_run_out_are_seen(attn, dtype, mode, D, prefix, nodes):
     assert torch.isnan(own[:total]).all() and (own[total:] == 0).all()
     again = c.run(attn, q=q, out=out)
     c.check(again[:total])
+
+
+@pytest.mark.parametrize("dtype,mode", [(BF16, "int8_per_token_head"), (F16, "int8_per_token_head"),
+                                        (BF16, "fp8_per_token_head"), (F16, "fp8_per_token_head"),
+                                        (F32, "int8_per_token_head")])
+@pytest.mark.parametrize("prefix", [0, 40, 700])
+@pytest.mark.parametrize("log2", [14, 24, 60, 110])
+@pytest.mark.parametrize("D", [64, 128])
+def test_hidden_value_scales_of_any_size(attn, dtype, mode, prefix, log2, D):
+    """A node whose (finite) value scale is 2^14 to 2^110 times the others' does not reach the rows
+    that do not see it: they are as exact as without it."""
+    n, big = 12, 5
+    visible = [[{0, j} for j in range(n)]]
+    c = Case(30, [prefix], [n], 8, 2, D, 16, dtype, mode, visible=visible)
+    t = prefix + big
+    c.vs[int(c.bt[0, t // 16]), t % 16] *= 2.0 ** log2
+    got = c.run(attn).clone()
+    c.visible[0][big] = {0}  # the row that sees it is left out of the check
+    ref, _, _ = c.ref()
+    got[big] = ref[big].to(dtype)
+    c.check(got)
+
+
+@pytest.mark.parametrize("dtype,mode", [(BF16, "int8_per_token_head"), (F16, "fp8_per_token_head")])
+@pytest.mark.parametrize("log2", [16, 30, 60, 100])
+@pytest.mark.parametrize("at", [3, 500, 1020, 2040])
+@pytest.mark.parametrize("D", [64, 128])
+def test_value_scales_of_tokens_that_weigh_nothing(attn, dtype, mode, log2, at, D):
+    """A token that every row sees, whose value scale is 2^log2 times the others' and whose weight
+    is so small that it hardly counts: the outputs are the others' values."""
+    c = Case(31, [2035], [9], 8, 2, D, 16, dtype, mode)
+    page, row = int(c.bt[0, at // 16]), at % 16
+    # queries of one sign, and a key against them: the score is lower by 2 log2 in the exponent of 2
+    c.q = c.q.abs() * 0.05
+    ones = torch.ones(c.k.shape[-1], device=DEV)
+    c.k[page, row] = (-ones * (100 if mode.startswith("int8") else 240)).to(c.k.dtype)
+    s = (c.q.float().sum(-1).amin() * c.scale * (100 if mode.startswith("int8") else 240)).item()
+    c.ks[page, row] = 1.5 * log2 * math.log(2) / s
+    c.vs[page, row] *= 2.0 ** log2
+    c.check(c.run(attn))
+
+
+@pytest.mark.parametrize("mode", ["int8_per_token_head", "fp8_per_token_head"])
+@pytest.mark.parametrize("first,last", [(2.0 ** 60, 2.0 ** -60), (2.0 ** -60, 2.0 ** 60), (2.0 ** 30, 2.0 ** -80)])
+def test_value_scales_from_tile_to_tile(attn, mode, first, last):
+    """Value scales that differ by up to 2^120 between the first and the last part of the context."""
+    c = Case(32, [1500, 70], [11, 3], 8, 2, 128, 16, BF16, mode)
+    for b, cut in ((0, 64), (1, 2)):
+        pages = c.bt[b].long()
+        c.vs[pages[:cut]] *= first
+        c.vs[pages[cut:-(-int(c.lens[b]) // 16)]] *= last
+    c.check(c.run(attn))
