@@ -523,7 +523,8 @@ MKV_API int mkv_tree_metadata(const void* parents, int32_t parents_index_type, c
  * K/V that a row does not see may hold anything (infinities and NaN included).
  * Caches: the query's dtype (bf16, f16, f32), FP8_E4M3 with k_scale / v_scale (one float
  * each) or with k_scales / v_scales per (page, row, kv head), INT8 with k_scales /
- * v_scales. head_dim is a multiple of 16, at most 256. query rows may have any strides
+ * v_scales. head_dim is a multiple of 16, at most 256; max_num_blocks * block_size is at most
+ * 2^31 - 1024. query rows may have any strides
  * (head_dim contiguous). workspace: 16-byte aligned, at least
  * mkv_paged_tree_workspace_bytes(...), its contents on entry do not matter; calls that may
  * overlap on the GPU need workspaces of their own.

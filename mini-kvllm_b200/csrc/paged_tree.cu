@@ -394,8 +394,9 @@ int tree_attention(const char* fn, bool zero_rest, TREE_PARAMETERS) {
     return set_error(MKV_ERR_INVALID_ARGUMENT, "%s: num_heads must be a multiple of num_kv_heads", fn);
   if (head_dim % 16 != 0 || head_dim > 256)
     return set_error(MKV_ERR_UNSUPPORTED, "%s: head_dim must be a multiple of 16, at most 256 (got %d)", fn, head_dim);
-  if ((int64_t)max_num_blocks * block_size > 0x7fffff00ll)
-    return set_error(MKV_ERR_UNSUPPORTED, "%s: max_num_blocks x block_size exceeds 2^31 tokens", fn);
+  // (token indices are 32-bit, and are formed for the three tiles of 128 behind a context's last one too)
+  if ((int64_t)max_num_blocks * block_size > 0x7fffffffll - 1023)
+    return set_error(MKV_ERR_UNSUPPORTED, "%s: max_num_blocks x block_size exceeds 2^31 tokens (less 1024)", fn);
   if (total_q > 0x7fffffffll / (num_heads / num_kv_heads))
     return set_error(MKV_ERR_UNSUPPORTED, "%s: total_q x query heads per kv head exceeds 2^31", fn);
   if (q_dtype != MKV_DTYPE_F32 && q_dtype != MKV_DTYPE_F16 && q_dtype != MKV_DTYPE_BF16)

@@ -60,7 +60,7 @@ static __device__ __noinline__ Seq load_seq(const Params& p, int b) {
   s.q0 = a;
   s.nodes = e > a ? (int)(e - a) : 0;
   const int64_t ctx = ld_idx(p.ctx, p.ctx_i64, b);
-  const int64_t cap = (int64_t)p.max_blocks * p.block_size;  // at most 2^31 - 1 (checked on the host)
+  const int64_t cap = (int64_t)p.max_blocks * p.block_size;  // at most 2^31 - 1024 (checked on the host)
   s.len = (int)max(min(ctx, cap), (int64_t)0);
   s.prefix = (int)max(min(ctx - s.nodes, (int64_t)s.len), (int64_t)0);
   return s;

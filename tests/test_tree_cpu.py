@@ -210,3 +210,15 @@ def test_the_limit_of_waits():
     assert lib.mkv_set_wait_limit(-5) == 123  # below 0 counts as 0
     assert lib.mkv_set_wait_limit(first) == 0
     assert lib.mkv_set_wait_limit(first) == first
+
+
+def test_tables_near_2_31_tokens():
+    """Indices of tokens are 32-bit in the kernels, which look up to three tiles of 128 past the tile
+    that holds the last token: a table must end 128 + 3 * 128 tokens before 2^31 at the least."""
+    lib = lib_mod.load()
+    for blocks, bs in (((1 << 31) // 256 - 2, 256), ((1 << 31) // 8 - 65, 8), ((1 << 31) - 512, 1), ((1 << 31) - 1023, 1)):
+        assert _tree(lib, maxb=blocks, bs=bs, wsb=1000) == 2 and b"2^31 tokens" in lib.mkv_last_error()
+    for blocks, bs in (((1 << 31) // 256 - 4, 256), ((1 << 31) - 1024, 1)):  # past this check, on to the next one
+        assert _tree(lib, maxb=blocks, bs=bs, wsb=1000) == 3
+        last = blocks * bs - 1
+        assert (last // 128 + 1) * 128 - 1 + 3 * 128 < 2 ** 31
