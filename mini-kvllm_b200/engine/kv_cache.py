@@ -233,6 +233,16 @@ def _indices(fn: str, what: str, t: torch.Tensor, dim: int) -> torch.Tensor:
     return t if t.is_contiguous() else t.contiguous()
 
 
+def _count(fn: str, t: Optional[torch.Tensor], idx: int) -> int:
+    """The address of a caller's count of skipped entries (0: none is kept)."""
+    if t is None:
+        return 0
+    if t.dtype != torch.int32 or t.numel() != 1 or t.get_device() != idx:
+        raise ValueError(f"{fn}: invalid_count must be one int32 on the same device, got {t.dtype} "
+                         f"{tuple(t.shape)} on {t.device}")
+    return t.data_ptr()
+
+
 def _tree_args(fn: str, parents, cu_seqlens_q, prefix_lens, block_tables, block_size):
     """(checked tensors, the argument list that the tree entry points share)"""
     parents = _indices(fn, "parents", parents, 1)
@@ -258,18 +268,25 @@ def _tree_args(fn: str, parents, cu_seqlens_q, prefix_lens, block_tables, block_
 
 
 def tree_metadata(parents: torch.Tensor, cu_seqlens_q: torch.Tensor, prefix_lens: torch.Tensor,
-                  block_tables: torch.Tensor, block_size: int, max_nodes: int) -> TreeMetadata:
+                  block_tables: torch.Tensor, block_size: int, max_nodes: int,
+                  invalid_count: Optional[torch.Tensor] = None) -> TreeMetadata:
     """Metadata of a decode step over trees of drafted tokens, in one kernel. parents
     (total_q,) holds each node's parent within its own tree (a lower index, -1 for a root),
     sequence b's nodes being rows [cu_seqlens_q[b], cu_seqlens_q[b+1]); prefix_lens[b] tokens
     are cached before them. Node i is cached at position prefix_lens[b] + i
     (slot_mapping, -1 without a page), sits at position prefix_lens[b] + its depth
     (positions) and sees itself and its ancestors (tree_mask). max_nodes bounds every tree
-    (at most 1024). Rows of no sequence get slot -1, which the append skips."""
+    (at most 1024). Rows of no sequence get slot -1, which the append skips.
+
+    A tree that breaks these rules is not seen on the host. A parent that is no lower node
+    counts as -1; a node past max_nodes (rounded up to 64) gets slot -1, so it is not cached,
+    and sees nothing. The number of both is added to invalid_count (one int32 on the device)
+    where that is given."""
     fn = "tree_metadata"
     if not 1 <= max_nodes <= 1024:
         raise ValueError(f"{fn}: max_nodes must be 1 to 1024 (got {max_nodes})")
     idx = _device_index(fn, parents, cu_seqlens_q, prefix_lens, block_tables)
+    bad = _count(fn, invalid_count, idx)
     keep, args = _tree_args(fn, parents, cu_seqlens_q, prefix_lens, block_tables, block_size)
     B, total, words, dev = args[-2], args[-1], (max_nodes + 63) // 64, parents.device
     slots = torch.empty(total, dtype=torch.int64, device=dev)
@@ -277,7 +294,7 @@ def tree_metadata(parents: torch.Tensor, cu_seqlens_q: torch.Tensor, prefix_lens
     positions = torch.empty(total, dtype=torch.int64, device=dev)
     mask = torch.empty(total, words, dtype=torch.int64, device=dev)
     st = _call_packed(_lib.load(), idx, _lib.CALL_TREE_METADATA, _lib.PACK_TREE_METADATA, args + (
-        words, slots.data_ptr(), lens.data_ptr(), positions.data_ptr(), mask.data_ptr(), 0))
+        words, slots.data_ptr(), lens.data_ptr(), positions.data_ptr(), mask.data_ptr(), bad))
     if st:
         _lib.check(fn, st)
     return TreeMetadata(slots, lens, positions, mask)
@@ -291,7 +308,8 @@ def tree_accept(draft_tokens: torch.Tensor, target_tokens: torch.Tensor, parents
     (target_tokens[row], e.g. the argmax or the sample of the row's logits), at most max_path
     nodes. Returns the path, its target tokens (the step's new tokens), the number of cached
     tokens to keep, and the moves that bring the accepted rows there (move_kv_rows). The
-    other arguments as for tree_metadata."""
+    other arguments as for tree_metadata, whose rules hold for the trees (a node that it did
+    not cache must not be accepted: its count tells)."""
     fn = "tree_accept"
     idx = _device_index(fn, draft_tokens, target_tokens, parents, cu_seqlens_q, prefix_lens, block_tables)
     draft, target = _indices(fn, "draft_tokens", draft_tokens, 1), _indices(fn, "target_tokens", target_tokens, 1)
@@ -346,31 +364,35 @@ def _pairs(fn: str, cache: KVCache, src: torch.Tensor, dst: torch.Tensor, dim: i
     return idx, src, dst
 
 
-def copy_kv_pages(cache: KVCache, src_pages: torch.Tensor, dst_pages: torch.Tensor) -> None:
+def copy_kv_pages(cache: KVCache, src_pages: torch.Tensor, dst_pages: torch.Tensor,
+                  invalid_count: Optional[torch.Tensor] = None) -> None:
     """Copies page src_pages[i] to page dst_pages[i] of every layer, K and V and the
     per-(token, head) scales, in one kernel: a forked sequence's own copy of a shared page,
     or the moves of a compaction. The copies are made in order, so one that reads a page
     written by an earlier one sees what was written; an entry below 0 is no copy, one past
-    the cache is skipped."""
+    the cache is skipped, and counted in invalid_count (one int32 on the device, added to)
+    where that is given."""
     fn = "copy_kv_pages"
     idx, src, dst = _pairs(fn, cache, src_pages, dst_pages, 1)
     st = _call_packed(_lib.load(), idx, _lib.CALL_COPY_KV_PAGES, _lib.PACK_COPY_PAGES, _cache_args(fn, cache) + (
-        src.data_ptr(), dst.data_ptr(), _INDEX[src.dtype], src.numel(), 0))
+        src.data_ptr(), dst.data_ptr(), _INDEX[src.dtype], src.numel(), _count(fn, invalid_count, idx)))
     if st:
         _lib.check(fn, st)
 
 
-def move_kv_rows(cache: KVCache, src_slots: torch.Tensor, dst_slots: torch.Tensor) -> None:
+def move_kv_rows(cache: KVCache, src_slots: torch.Tensor, dst_slots: torch.Tensor,
+                 invalid_count: Optional[torch.Tensor] = None) -> None:
     """Copies the cached row of slot src_slots[g, i] to slot dst_slots[g, i] in every layer,
     K and V and the per-(token, head) scales, in one kernel: the accepted rows of a tree,
     moved to the end of the cached prefix (tree_accept gives the slots). Moves are made in
     order within a group g (a sequence); the groups run side by side, so what one of them
     writes no other may read or write. An entry below 0 is no move, one past the cache is
-    skipped."""
+    skipped, and counted in invalid_count as by copy_kv_pages."""
     fn = "move_kv_rows"
     idx, src, dst = _pairs(fn, cache, src_slots, dst_slots, 2)
     st = _call_packed(_lib.load(), idx, _lib.CALL_MOVE_KV_ROWS, _lib.PACK_MOVE_ROWS, _cache_args(fn, cache) + (
-        src.data_ptr(), dst.data_ptr(), _INDEX[src.dtype], src.shape[0], src.shape[1], 0))
+        src.data_ptr(), dst.data_ptr(), _INDEX[src.dtype], src.shape[0], src.shape[1],
+        _count(fn, invalid_count, idx)))
     if st:
         _lib.check(fn, st)
 

@@ -222,3 +222,11 @@ def test_tables_near_2_31_tokens():
         assert _tree(lib, maxb=blocks, bs=bs, wsb=1000) == 3
         last = blocks * bs - 1
         assert (last // 128 + 1) * 128 - 1 + 3 * 128 < 2 ** 31
+
+
+def test_counts_are_one_int32_on_the_device():
+    one = torch.zeros(1, dtype=torch.int32)
+    assert kv._count("f", None, 0) == 0 and kv._count("f", one, -1) == one.data_ptr()
+    for t, idx in ((one, 0), (one.long(), -1), (torch.zeros(2, dtype=torch.int32), -1)):
+        with pytest.raises(ValueError, match="invalid_count"):
+            kv._count("f", t, idx)

@@ -482,3 +482,28 @@ def test_packed_calls_refuse():
     lib = lib_mod.load()
     assert lib.mkv_call_packed(5, b"\0" * 400) == 1 and b"unknown call" in lib.mkv_last_error()
     assert lib.mkv_call_packed(0, None) == 1 and b"null pointer" in lib.mkv_last_error()
+
+
+def test_invalid_entries_are_counted(kv):
+    """Trees that are none, trees wider than their masks, and copies past the cache can be noticed
+    through the public functions; the results are those without the count."""
+    bad = dev([5], torch.int32)  # it is added to
+    parents, cu = [-1, 0, 7, 1, -9] + list(range(-1, 69)), [0, 5, 75]
+    args = (dev(parents, torch.int32), dev(cu), dev([3, 0]), dev([[4, 1], [3, 2]], torch.int32), 16)
+    a, b = kv.tree_metadata(*args, 64), kv.tree_metadata(*args, 64, invalid_count=bad)
+    assert bad.tolist() == [5 + 2 + 6]  # parents 7 and -9; nodes 64 to 69
+    for x, y in zip((a.slot_mapping, a.context_lens, a.positions, a.tree_mask),
+                    (b.slot_mapping, b.context_lens, b.positions, b.tree_mask)):
+        assert torch.equal(x, y)
+    kv.tree_metadata(*args, 70, invalid_count=bad)
+    assert bad.tolist() == [15]
+    c, want = (cache_of(kv, "auto") for _ in range(2))
+    pages_ref(want, [1, 11, 3, -1], [2, 4, 1 << 20, 5])
+    kv.copy_kv_pages(c, dev([1, 11, 3, -1]), dev([2, 4, 1 << 20, 5]), invalid_count=bad.zero_())
+    assert bad.tolist() == [2]
+    rows_ref(want, [[1, -1], [176, 7]], [[0, 3], [5, 8]])
+    kv.move_kv_rows(c, dev([[1, -1], [176, 7]]), dev([[0, 3], [5, 8]]), invalid_count=bad)
+    assert bad.tolist() == [3]
+    assert torch.equal(planes(c)[0], planes(want)[0])
+    with pytest.raises(ValueError, match="invalid_count"):
+        kv.copy_kv_pages(c, dev([1]), dev([2]), invalid_count=torch.zeros(1, dtype=torch.int32))
