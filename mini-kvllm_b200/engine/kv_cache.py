@@ -260,8 +260,8 @@ def _tree_args(fn: str, parents, cu_seqlens_q, prefix_lens, block_tables, block_
     B = prefix.numel()
     if cu.numel() != B + 1 or rows < B:
         raise ValueError(f"{fn}: cu_seqlens_q/block_tables do not match {B} sequences")
-    if block_size <= 0:
-        raise ValueError(f"{fn}: block_size must be positive")
+    if not 0 < block_size < 1 << 31:  # (32 bits in the C call)
+        raise ValueError(f"{fn}: block_size must be positive and below 2^31 (got {block_size})")
     return (parents, cu, prefix, tables), (
         parents.data_ptr(), _INDEX[parents.dtype], cu.data_ptr(), _INDEX[cu.dtype], prefix.data_ptr(),
         _INDEX[prefix.dtype], tables.data_ptr(), tt, stride[0], width, block_size, B, parents.numel())
@@ -311,14 +311,14 @@ def tree_accept(draft_tokens: torch.Tensor, target_tokens: torch.Tensor, parents
     other arguments as for tree_metadata, whose rules hold for the trees (a node that it did
     not cache must not be accepted: its count tells)."""
     fn = "tree_accept"
+    if not 1 <= max_path < 1 << 31:  # (32 bits in the C call)
+        raise ValueError(f"{fn}: max_path must be at least 1 and below 2^31 (got {max_path})")
     idx = _device_index(fn, draft_tokens, target_tokens, parents, cu_seqlens_q, prefix_lens, block_tables)
     draft, target = _indices(fn, "draft_tokens", draft_tokens, 1), _indices(fn, "target_tokens", target_tokens, 1)
     keep, args = _tree_args(fn, parents, cu_seqlens_q, prefix_lens, block_tables, block_size)
     B, total = args[-2], args[-1]
     if draft.numel() != total or target.numel() != total or draft.dtype != target.dtype:
         raise ValueError(f"{fn}: draft_tokens and target_tokens must be {total} tokens each, of one dtype")
-    if max_path < 1:
-        raise ValueError(f"{fn}: max_path must be at least 1 (got {max_path})")
     dev = parents.device
     tokens = torch.empty(B, max_path, dtype=torch.int64, device=dev)
     src, dst = torch.empty_like(tokens), torch.empty_like(tokens)

@@ -230,3 +230,13 @@ def test_counts_are_one_int32_on_the_device():
     for t, idx in ((one, 0), (one.long(), -1), (torch.zeros(2, dtype=torch.int32), -1)):
         with pytest.raises(ValueError, match="invalid_count"):
             kv._count("f", t, idx)
+
+
+@pytest.mark.parametrize("size", [0, -16, 1 << 31, (1 << 32) + 16])
+def test_sizes_that_do_not_fit_the_c_call(size):
+    """They are refused, not cut to 32 bits ((1 << 32) + 16 would be read as 16)."""
+    par, cu, pre, bt = torch.zeros(3, dtype=torch.int32), torch.tensor([0, 3]), torch.tensor([4]), torch.zeros(1, 4).int()
+    with pytest.raises(ValueError, match="block_size"):
+        kv._tree_args("f", par, cu, pre, bt, size)
+    with pytest.raises(ValueError, match="max_path"):
+        kv.tree_accept(par, par, par, cu, pre, bt, 16, size)
