@@ -586,7 +586,8 @@ MKV_API int mkv_tree_accept(const void* draft_tokens, const void* target_tokens,
 
 /*
  * Copies inside the cache, over all layers, K and V and (when given) the per-(page, row, kv
- * head) scales, in one launch. k_cache / v_cache point at layer 0, (num_blocks, block_size,
+ * head) scales, in one launch (many copies of small pages or rows in one for each 1024 of them).
+ * k_cache / v_cache point at layer 0, (num_blocks, block_size,
  * num_kv_heads, head_dim) each, layer_stride elements from layer to layer; k_scales /
  * v_scales likewise (num_blocks, block_size, num_kv_heads), scale_layer_stride apart, or
  * both NULL. A token's row (num_kv_heads x head_dim values) must be a multiple of 16 bytes.

@@ -1,6 +1,6 @@
 // Copies of cached data inside the paged KV cache, over every layer, K and V and the row
-// scales in one launch: whole pages (a fork's private copy of a shared page, compaction of
-// a fragmented cache) and single rows (the accepted rows of a tree of drafted tokens,
+// scales in one launch (several, one for each 1024 pairs, where the pairs are split): whole pages (a
+// fork's private copy of a shared page, compaction of a fragmented cache) and single rows (the accepted rows of a tree of drafted tokens,
 // moved to the end of the cached prefix).
 //
 // A copy moves `unit` bytes (a page, or one token's row of all kv heads) from unit src[i]
@@ -13,8 +13,9 @@
 // at a time.
 //
 // Bound: memory, 2 x unit bytes a copy. The columns of a whole cache (28 layers of 32 KB
-// pages: 114688) keep 14 MB in flight, enough to cover the latency of HBM, and their threads
-// fit the GPU at once (233 pairs: 140 us, 6.1 TB/s, 0.94 of the copy rate; three pairs 3.4 us).
+// pages: 114688, two layers to a thread) keep 57344 threads x 128 bytes = 7.3 MB in flight, enough
+// to cover the latency of HBM, and the threads fit the GPU at once (233 pairs: 140 us, 6.1 TB/s, 0.94
+// of the copy rate; three pairs 3.4 us).
 // Where the columns are few and the pairs many (small pages of one kv head), the pairs are split
 // over CTAs as well, if none of them writes what another one reads or writes: every CTA finds
 // that out for itself, with a hash table of the destinations.

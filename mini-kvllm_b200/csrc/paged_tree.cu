@@ -23,8 +23,9 @@ namespace {
 // Every type and head_dim (a multiple of 16, at most 256): 16 rows x 32 tokens per step in
 // fp32. A warp owns 4 rows; lane = token for the scores, lane = column for the products. Bound by
 // shared memory (5 16-byte loads to 16 products a lane) and, with few rows, by the latency of a
-// tile, which four CTAs an SM cover: fp32, 8 x 4k tokens, 32 rows a kv head 418 us (2 CTAs: 725).
-// 8 rows a warp have fewer loads per product, but their registers halve the CTAs (479).
+// tile, which four CTAs an SM cover: fp32, 8 sequences of 3-4k tokens, 16 to 32 rows on each of 8 kv
+// heads 418 us (2 CTAs: 725); 8 x 4k tokens, 32 rows on each 509 us, 13 times what its bytes take.
+// 8 rows a warp have fewer loads per product, but their registers halve the CTAs (479 for 418).
 constexpr int kGRows = 16, kGKT = 32, kGThreads = 128;
 constexpr int kGCtas = 4 * kNumSMs;  // resident with head_dim up to 128
 

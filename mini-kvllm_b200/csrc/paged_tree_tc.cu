@@ -17,12 +17,14 @@
 // padded, which costs nothing while the tile's bytes take longer to arrive (bf16: 64 KB a
 // tile, 1.5 us of an SM's share of HBM; its two products 0.55 us).
 //
-// Measured (B200, device time of the call with its combine): bf16, 48 sequences of 1-8k tokens, 8-32
-// nodes, 32/8 heads 172 us, 5.42 TB/s (0.83 of the copy rate), DRAM reads 0.94 GB = K and V once;
-// e4m3, 12 x 32k, 32 nodes 246 us, 838 TFLOP/s, tensor pipe 39 % and exponentials 39 % busy: a tile
-// takes 2500 clocks, of them 1050 each for the exponentials, the products and (four warps) the
-// conversions, in a chain that two streams overlap by half; int8 with row scales, 19 x 1-5k over
-// 16-token pages 77 us. Two streams, not one shared accumulator or half a tile per warpgroup: both
+// Measured (B200, device time of the call with its combine, short replays): bf16, 48 sequences of
+// 1-8k tokens, 8-32 nodes, 32/8 heads 168-172 us, 5.4 TB/s (0.83 of the copy rate; 201 us where calls
+// follow one another for seconds, under the power cap), DRAM reads 0.94 GB = K and V once; e4m3,
+// 12 x 32k, 32 nodes 241-246 us, 840 TFLOP/s, tensor pipe 40 % and exponentials 40 % busy: a tile
+// takes 2500 clocks; the MMA issuer is busy for 1375 of them, the converters for 2100 (890 convert,
+// the rest are fences, arrivals and table lookups), the exponentials take 1050, in a chain that two
+// streams overlap by half; int8 with row scales, 19 x 1-5k over 16-token pages 78 us: 2.0 us a tile
+// (24 a CTA) and 28 us outside the tiles. Two streams, not one shared accumulator or half a tile per warpgroup: both
 // measured slower (250-270 us against 319 and 391 for e4m3).
 //
 // What a row must not see: scores of hidden tokens are replaced by -inf before the maximum.
@@ -137,7 +139,9 @@ paged_tree_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ C
   constexpr int TILE = L::TILE;
   using MT = typename std::conditional<kByte, f16, QT>::type;  // operands of the MMAs
   // f16 weights: 2^6 above the reference, so that they stay normal down to 2^-20 of the
-  // largest; with the lazy reference (2^8) and a scale factor below 2 they end below 2^15.
+  // largest (below 2^-31 of it they are 0: up to that times the value is lost of a token, which
+  // counts where the heavy tokens' values are 0); with the lazy reference (2^8) and a scale factor
+  // below 2 they end below 2^15.
   constexpr float kBias = std::is_same<MT, f16>::value ? 6.0f : 0.0f;
   constexpr bool kToF16 = kByte && std::is_same<QT, bf16>::value;  // Q changes its type
   constexpr int kKS = L::kKS, kVS = L::kVS, kRS = kByte ? L::kRS : 1;

@@ -367,7 +367,7 @@ def _pairs(fn: str, cache: KVCache, src: torch.Tensor, dst: torch.Tensor, dim: i
 def copy_kv_pages(cache: KVCache, src_pages: torch.Tensor, dst_pages: torch.Tensor,
                   invalid_count: Optional[torch.Tensor] = None) -> None:
     """Copies page src_pages[i] to page dst_pages[i] of every layer, K and V and the
-    per-(token, head) scales, in one kernel: a forked sequence's own copy of a shared page,
+    per-(token, head) scales, in one call: a forked sequence's own copy of a shared page,
     or the moves of a compaction. The copies are made in order, so one that reads a page
     written by an earlier one sees what was written; an entry below 0 is no copy, one past
     the cache is skipped, and counted in invalid_count (one int32 on the device, added to)
@@ -383,7 +383,7 @@ def copy_kv_pages(cache: KVCache, src_pages: torch.Tensor, dst_pages: torch.Tens
 def move_kv_rows(cache: KVCache, src_slots: torch.Tensor, dst_slots: torch.Tensor,
                  invalid_count: Optional[torch.Tensor] = None) -> None:
     """Copies the cached row of slot src_slots[g, i] to slot dst_slots[g, i] in every layer,
-    K and V and the per-(token, head) scales, in one kernel: the accepted rows of a tree,
+    K and V and the per-(token, head) scales, in one call: the accepted rows of a tree,
     moved to the end of the cached prefix (tree_accept gives the slots). Moves are made in
     order within a group g (a sequence); the groups run side by side, so what one of them
     writes no other may read or write. An entry below 0 is no move, one past the cache is
