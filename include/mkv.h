@@ -530,8 +530,9 @@ MKV_API int mkv_tree_metadata(const void* parents, int32_t parents_index_type, c
  * overlap on the GPU need workspaces of their own.
  * The warps of a thread block hand tiles to each other and wait no longer than a limit for one;
  * a block that meets it makes every row that it has a part in NaN. mkv_set_wait_limit sets the
- * limit for the calls that follow, in GPU clocks, and returns the last one (2e9, about a second,
- * where none was set; a debugger that stops single warps needs more; 0 lets no wait succeed).
+ * limit for the calls that follow (a captured one keeps its own), in GPU clocks, and returns the
+ * last one (2e9, about a second, where none was set; a debugger that stops single warps needs more;
+ * 0 lets no wait succeed).
  */
 MKV_API int64_t mkv_set_wait_limit(int64_t clocks);
 MKV_API size_t mkv_paged_tree_workspace_bytes(int32_t num_seqs, int64_t total_q, int32_t num_heads,

@@ -300,7 +300,9 @@ paged_tree_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ C
     }
     if (!ok) *abort_flag = 1;
     __syncwarp();
-    if (lane == 0 && *abort_flag) {  // loads in flight land before the CTA exits
+    // loads in flight land before the CTA goes on to its end, whichever role gives up, and when (in a call
+    // that runs well the last tile's products wait for the same loads)
+    if (lane == 0) {
       if constexpr (kByte) {
         for (uint32_t k = nk > kRS ? nk - kRS : 0; k < nk; ++k) mbar_wait(&rfull[k % kRS], (k / kRS) & 1, nullptr);
       } else {

@@ -240,3 +240,18 @@ def test_sizes_that_do_not_fit_the_c_call(size):
         kv._tree_args("f", par, cu, pre, bt, size)
     with pytest.raises(ValueError, match="max_path"):
         kv.tree_accept(par, par, par, cu, pre, bt, 16, size)
+
+
+def test_loads_in_flight_are_waited_for_whoever_gives_up():
+    """A block whose wait has run out uses its shared memory again, so no load may still be on its way
+    there: the producer's last waits do not ask whether anyone has given up (another warp may do so
+    later), and the issuer of the products waits for them the same way."""
+    import pathlib
+    import re
+    code = (pathlib.Path(lib_mod.PKG_DIR) / "csrc" / "paged_tree_tc.cu").read_text()
+    for what in (r"mbar_wait\(&rfull\[k % kRS\], \(k / kRS\) & 1, nullptr\)", r"mbar_wait\(&kfull\[k % kKS\], \(k / kKS\) & 1, nullptr\)",
+                 r"mbar_wait\(&vfull\[k % kVS\], \(k / kVS\) & 1, nullptr\)", r"mbar_wait\(drain, 0, nullptr\)"):
+        at = [m.start() for m in re.finditer(what, code)]
+        assert len(at) == 1, what
+        guards = re.findall(r"if \(([^{};]*)\) \{", code[code.rindex("if (!ok) *abort_flag = 1;", 0, at[0]):at[0]])
+        assert guards and not any("abort" in g for g in guards), guards
