@@ -628,3 +628,47 @@ def test_value_scales_from_tile_to_tile(attn, mode, first, last):
         c.vs[pages[:cut]] *= first
         c.vs[pages[cut:-(-int(c.lens[b]) // 16)]] *= last
     c.check(c.run(attn))
+
+
+@pytest.mark.parametrize("mode", ["auto", "int8_per_token_head"])
+def test_replays_of_a_padded_batch_whose_trees_change(attn, mode):
+    """One captured call of fixed sizes, replayed on batches of other lengths, trees and numbers of
+    sequences: what was padding in one replay is a row of the next, and the other way round."""
+    B, total, words = 5, 60, 1
+    cases = [Case(40 + i, p, n, 8, 2, 128, 16, BF16, mode) for i, (p, n) in enumerate((
+        ([50, 0, 700, 3, 9], [4, 1, 40, 10, 5]), ([1500], [3]), ([0, 20], [0, 60]), ([400, 5, 5], [1, 1, 1])))]
+    NB = max(c.k.shape[0] for c in cases)
+    k, v = (torch.zeros(NB, 16, 2, 128, dtype=cases[0].k.dtype, device=DEV) for _ in range(2))
+    ks, vs = (torch.zeros(NB, 16, 2, device=DEV) if mode != "auto" else None for _ in range(2))
+    q = torch.zeros(total, 8, 128, dtype=BF16, device=DEV)
+    bt = torch.full((B, 130), -1, dtype=torch.int32, device=DEV)
+    lens, cu = torch.zeros(B, dtype=torch.int64, device=DEV), torch.zeros(B + 1, dtype=torch.int32, device=DEV)
+    mask = torch.zeros(total, words, dtype=torch.int64, device=DEV)
+
+    def fill(c):
+        n, b = c.cu[-1], c.B
+        k[:c.k.shape[0]], v[:c.k.shape[0]] = c.k, c.v
+        if ks is not None:
+            ks[:c.k.shape[0]], vs[:c.k.shape[0]] = c.ks, c.vs
+        q[:n], q[n:] = c.q, float("nan")
+        bt.fill_(-1)
+        bt[:b, :c.bt.shape[1]] = c.bt
+        lens.zero_(), mask.fill_(-1)
+        lens[:b], mask[:n] = c.lens, c.mask
+        cu[:b + 1], cu[b + 1:] = c.cut, n
+
+    def call():
+        return attn.paged_attention_tree(q, k, v, bt, lens, cu, mask, cases[0].scale, 8, 2, 128, 16, ks, vs, mode)
+
+    fill(cases[0])
+    call()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call()
+    for c in cases + cases[::-1]:
+        fill(c)
+        out.fill_(float("nan"))
+        graph.replay()
+        n = c.cu[-1]
+        c.check(out[:n])
+        assert (out[n:] == 0).all()
